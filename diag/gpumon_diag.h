@@ -193,6 +193,82 @@ GMD_API int gmd_gemm_launch_mx(const void* a, const void* b, const void* scale_a
                                int m, int n, int k, void* hip_stream);
 GMD_API int gmd_mx_pack_scales(const void* scales_row_major, void* packed, int rows, int k, void* hip_stream);
 
+/* ------------------------------------- fp8 in blocks of 128, and GEMMs by expert -- */
+/* e4m3 with one f32 scale per block of 128: what a mixture-of-experts job feeds its products.  All launches below work on
+ * caller memory of the current device, are asynchronous in `hip_stream`, need no workspace, read nothing back to the host
+ * and can be captured into a graph.  A stride of 0 means packed.  A size of zero is no error. */
+typedef enum {
+  GMD_BLOCK_ROWS = 0,  /* 128 consecutive elements of a row share a scale; scales[kb * ld_scales + row] */
+  GMD_BLOCK_TILES = 1  /* 128 x 128 elements do;                          scales[(row / 128) * ld_scales + kb] */
+} gmd_block_t;
+
+/* Quantises src [rows, cols] (bf16 or f32), or with `transpose` src^T [cols, rows], to e4m3 [r, c]:
+ *   amax = max |x| over the block, at least 2^-96;  scale = f32(amax / 448);  q = e4m3(f32(x * f32(448 / amax)))
+ * rounded to nearest, ties to even.  The result's rows are filled up to the next multiple of 16 with zeros (ld_dst is a
+ * multiple of 16, dst 16-byte aligned); blocks at the end of a row or at the bottom may be partial.  A block holding an
+ * infinity or a NaN gets an infinite or NaN scale, so that every product that reads it is NaN.
+ * Any rows, cols and ld_src >= cols; src rows that are 16-byte aligned are read in 16-byte pieces. */
+typedef struct {
+  const void* src;
+  void* dst;
+  float* scales;
+  int64_t ld_src, ld_dst, ld_scales;  /* elements; 0 = cols, c rounded up to 16, r (rows) or ceil(c / 128) (tiles) */
+  int32_t rows, cols;                 /* of src */
+  int32_t src_dtype;                  /* GMD_DT_BF16 or GMD_DT_F32 */
+  int32_t blocks;                     /* gmd_block_t */
+  int32_t transpose;
+  int32_t reserved;
+} gmd_block_quantize_t;
+GMD_API int gmd_block_quantize_launch(const gmd_block_quantize_t* q, void* hip_stream);
+
+/* C[m, n] = sum over blocks kb of scale_a[kb][m] * scale_b(kb, n) * (sum over the block's k of A[m, k] * B[n, k])
+ * A [m, k] and B [n, k] e4m3, row-major; C row-major bf16 or f32.  A's blocks are rows; B's are tiles (a weight)
+ * or rows (a weight gradient: A = dy^T and B = x^T, both quantised along the tokens).
+ * Sums are held in f32.  Within a block, bf16 results use the fp8 matrix instruction, which drops the part of a product that
+ * lies below 2^-13 of the largest of its group of eight k (at most 2^-10 of the sum of magnitudes); f32 results use the bf16
+ * instruction on the widened elements, which keeps it, at half the rate.
+ * Any m, n a multiple of 8, k a multiple of 16 (the last block may be partial); operands 16-byte aligned, row strides in
+ * multiples of 16 bytes up to 8 MiB. */
+typedef struct {
+  const void *a, *b;
+  void* c;
+  const float *scale_a, *scale_b;
+  int64_t lda, ldb, ldc;             /* elements; 0 = k, k, n */
+  int64_t ld_scale_a, ld_scale_b;    /* floats; 0 = m, and ceil(k / 128) (tiles) or n (rows) */
+  int32_t m, n, k;
+  int32_t b_blocks;                  /* gmd_block_t */
+  int32_t out_dtype;                 /* GMD_DT_BF16 or GMD_DT_F32 */
+  int32_t reserved;
+} gmd_gemm_block_t;
+GMD_API int gmd_gemm_block_launch(const gmd_gemm_block_t* g, void* hip_stream);
+
+/* GEMMs grouped by expert.  Rows are sorted by expert: expert e owns rows offsets[e] .. offsets[e + 1] - 1 (int32, device
+ * memory, groups + 1 of them, ascending); `rows` is the capacity, rows outside every expert's range are left as they were.
+ * Offsets that are out of range or descend are clamped into [0, rows] (the result is then of no use, but nothing outside the
+ * operands is touched).  w is [groups][n, k].
+ *   forward  c [rows, n]      = a [rows, k] times b = w:  c[t, n] = sum over k of a[t, k] * w[e][n, k]
+ *   dgrad    c [rows, k]      = a = dy [rows, n] times b = w:  c[t, k] = sum over n of dy[t, n] * w[e][n, k]
+ *   wgrad    c [groups][n, k] = a = dy [rows, n], b = x [rows, k]:  c[e][n, k] = sum over e's rows of dy[t, n] * x[t, k]
+ *            (zeros for an expert without rows)
+ * bf16: n and k in multiples of 8.  fp8 (e4m3 in blocks of 128: a's blocks are rows, w's tiles): forward only, n a multiple
+ * of 8, k of 16; its input gradient is the forward with the weights quantised transposed.  Sums as in
+ * gmd_gemm_block_launch (bf16 operands: f32 throughout).  Operands 16-byte
+ * aligned, strides in multiples of 16 bytes, row strides up to 8 MiB. */
+typedef enum { GMD_GROUPED_FORWARD = 0, GMD_GROUPED_DGRAD = 1, GMD_GROUPED_WGRAD = 2 } gmd_grouped_op_t;
+typedef struct {
+  const void *a, *b;
+  void* c;
+  const int32_t* offsets;
+  const float *scale_a, *scale_b;    /* fp8: [ceil(k / 128)][rows] and [groups][ceil(n / 128)][ceil(k / 128)] */
+  int64_t lda, ldb, ldc;             /* elements between rows; 0 = packed */
+  int64_t stride_w;                  /* elements between experts of b (forward, dgrad) or c (wgrad); 0 = n rows */
+  int64_t ld_scale_a, ld_scale_b, stride_scale; /* floats; stride_scale between experts of scale_b; 0 = packed */
+  int32_t op, dtype, out_dtype;      /* gmd_grouped_op_t; GMD_DT_BF16 or GMD_DT_FP8; GMD_DT_BF16 or GMD_DT_F32 */
+  int32_t groups, rows, n, k;
+  int32_t reserved;
+} gmd_grouped_gemm_t;
+GMD_API int gmd_grouped_gemm_launch(const gmd_grouped_gemm_t* g, void* hip_stream);
+
 /* GEMM schedule: -1 = the fastest for the dtype and shape (default); 0 = simple double-buffered loop;
  * 1 = eight waves x 128x64, one workgroup per tile; 2 = four waves x 128x128 with the accumulators in AGPRs;
  * 3 = eight waves x 128x64 as one stream per CU over its tiles (needs more tiles than CUs and >= 4 K-tiles);

@@ -1,0 +1,105 @@
+// GEMMs grouped by expert: rows sorted by expert, expert e owning rows offsets[e] .. offsets[e + 1] - 1 (device memory).
+//   forward  c[t, n]    = sum over k of a[t, k] * b[e][n, k]          a = x,  b = W
+//   dgrad    c[t, k]    = sum over n of a[t, n] * b[e][n, k]          a = dy, b = W
+//   wgrad    c[e][n, k] = sum over e's rows t of a[t, n] * b[t, k]    a = dy, b = x
+// One launch for all experts; nothing is read back to the host and no workspace is needed, so a launch can be captured.
+#include "gemm_tiles.h"
+
+namespace gmd {
+namespace tiles {
+namespace {
+
+template <bool TA, bool TB, bool WGRAD, int BM, int BN, int WM, int WN, typename OUT>
+int launch_tile(const Args& p, hipStream_t st) {
+  const int64_t grid = WGRAD ? (int64_t)p.groups * ((p.m + BM - 1) / BM) * ((p.n + BN - 1) / BN) : grid_of(p, BM, BN);
+  if (int rc = launched("grouped GEMM", grid)) return rc;
+  tile_kernel<kBf16, TA, TB, WGRAD, BM, BN, WM, WN, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
+  GMD_HIP(hipGetLastError());
+  return GMD_OK;
+}
+
+template <int MB, typename OUT>
+int launch_few(const Args& p, hipStream_t st) {
+  const int64_t grid = grid_of(p, MB * 16, 16);
+  if (int rc = launched("grouped GEMM", grid)) return rc;
+  few_rows_kernel<kBf16, MB, OUT><<<(unsigned)grid, kFewWaves * 64, 0, st>>>(p);
+  GMD_HIP(hipGetLastError());
+  return GMD_OK;
+}
+
+template <typename OUT>
+int launch_bf16(int op, const Args& p, hipStream_t st) {
+  const int rows = (p.m + p.groups - 1) / p.groups;  // an expert's share on average
+  if (op == GMD_GROUPED_FORWARD) {
+    if (rows <= 16) return launch_few<1, OUT>(p, st);
+    if (rows <= 32) return launch_few<2, OUT>(p, st);
+    if (rows <= 64) return launch_few<4, OUT>(p, st);
+    if (grid_of(p, 256, 256) >= kCUs) return launch_tile<false, false, false, 256, 256, 2, 4, OUT>(p, st);
+    return launch_tile<false, false, false, 128, 128, 2, 2, OUT>(p, st);
+  }
+  if (op == GMD_GROUPED_DGRAD) {
+    if (rows > 64 && grid_of(p, 256, 256) >= kCUs) return launch_tile<false, true, false, 256, 256, 2, 4, OUT>(p, st);
+    return launch_tile<false, true, false, 128, 128, 2, 2, OUT>(p, st);
+  }
+  if ((int64_t)p.groups * (p.m / 256) * (p.n / 256) >= kCUs) return launch_tile<true, true, true, 256, 256, 2, 4, OUT>(p, st);
+  return launch_tile<true, true, true, 128, 128, 2, 2, OUT>(p, st);
+}
+
+}  // namespace
+}  // namespace tiles
+}  // namespace gmd
+
+extern "C" {
+
+int gmd_grouped_gemm_launch(const gmd_grouped_gemm_t* g, void* hip_stream) {
+  using namespace gmd::tiles;
+  auto refuse = [](const char* why) {
+    gmd::set_error("grouped GEMM: %s", why);
+    return GMD_ERR_BADPARAM;
+  };
+  if (!g || g->rows < 0 || g->n < 0 || g->k < 0 || g->groups < 0) return refuse("negative sizes");
+  if (g->op != GMD_GROUPED_FORWARD && g->op != GMD_GROUPED_DGRAD && g->op != GMD_GROUPED_WGRAD) return refuse("op is forward, dgrad or wgrad");
+  if (g->dtype != GMD_DT_BF16 && g->dtype != GMD_DT_FP8) return refuse("operands are bf16 or fp8");
+  if (g->out_dtype != GMD_DT_BF16 && g->out_dtype != GMD_DT_F32) return refuse("the result is bf16 or f32");
+  const bool fp8 = g->dtype == GMD_DT_FP8, wgrad = g->op == GMD_GROUPED_WGRAD, dgrad = g->op == GMD_GROUPED_DGRAD;
+  if (fp8 && g->op != GMD_GROUPED_FORWARD)
+    return refuse("fp8 runs forward only: the input gradient is a forward with transposed weights, the weight gradient is taken in bf16");
+  if (g->n % 8 || g->k % (fp8 ? 16 : 8)) return refuse("N in multiples of 8, K in multiples of 8 (bf16) or 16 (fp8)");
+  if (g->n == 0 || g->groups == 0 || (g->k == 0 && g->op != GMD_GROUPED_FORWARD) || (g->rows == 0 && !wgrad)) return GMD_OK;
+  if (!g->offsets || ((uintptr_t)g->offsets & 3)) return refuse("null or misaligned offsets");
+
+  const int elem = fp8 ? 1 : 2, out = g->out_dtype == GMD_DT_BF16 ? 2 : 4;
+  const int64_t kb = ((int64_t)g->k + 127) / 128, nb = ((int64_t)g->n + 127) / 128;
+  const int64_t a_cols = g->op == GMD_GROUPED_FORWARD ? g->k : g->n;
+  const int64_t c_cols = g->op == GMD_GROUPED_FORWARD ? g->n : g->k;
+  const int64_t lda = g->lda ? g->lda : a_cols, ldb = g->ldb ? g->ldb : g->k, ldc = g->ldc ? g->ldc : c_cols;
+  const int64_t stride_w = g->stride_w ? g->stride_w : (int64_t)g->n * (wgrad ? ldc : ldb);
+  const char* bad = bad_operand(g->c, ldc * out, c_cols * out);
+  if (!bad && a_cols > 0 && g->rows > 0) bad = bad_operand(g->a, lda * elem, a_cols * elem);
+  if (!bad && g->k > 0 && (!wgrad || g->rows > 0)) bad = bad_operand(g->b, ldb * elem, (int64_t)g->k * elem);
+  if (!bad && (stride_w * (wgrad ? out : elem) % 16 || stride_w < (int64_t)(g->n - 1) * (wgrad ? ldc : ldb) + g->k))
+    bad = "an expert stride that is not a multiple of 16 bytes or shorter than an expert";
+  Args p;
+  memset(&p, 0, sizeof p);
+  p.a = (const char*)g->a, p.b = (const char*)g->b, p.c = g->c, p.offsets = g->offsets, p.groups = g->groups;
+  p.lda = lda * elem, p.ldb = ldb * elem, p.ldc = ldc;
+  if (wgrad) {
+    p.m = g->n, p.n = g->k, p.k = g->rows, p.stride_c = stride_w;
+  } else {
+    p.m = g->rows, p.n = dgrad ? g->k : g->n, p.k = dgrad ? g->n : g->k, p.stride_b = stride_w * elem;
+  }
+  if (fp8 && !bad && g->k > 0) {
+    p.sa = g->scale_a, p.sb = g->scale_b;
+    p.ld_sa = g->ld_scale_a ? g->ld_scale_a : g->rows;
+    p.ld_sb = g->ld_scale_b ? g->ld_scale_b : kb;
+    p.stride_sb = g->stride_scale ? g->stride_scale : nb * p.ld_sb;
+    if (!p.sa || !p.sb || (((uintptr_t)p.sa | (uintptr_t)p.sb) & 3)) bad = "null or misaligned scales";
+    else if (p.ld_sa < g->rows || p.ld_sb < kb || p.stride_sb < (nb - 1) * p.ld_sb + kb) bad = "a stride of scales shorter than what it spans";
+  }
+  if (bad) return refuse(bad);
+  if (fp8) return launch_fp8(p, GMD_BLOCK_TILES, g->out_dtype, (hipStream_t)hip_stream);
+  return g->out_dtype == GMD_DT_BF16 ? launch_bf16<__bf16>(g->op, p, (hipStream_t)hip_stream)
+                                     : launch_bf16<float>(g->op, p, (hipStream_t)hip_stream);
+}
+
+}  // extern "C"

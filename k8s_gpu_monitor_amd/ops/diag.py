@@ -91,6 +91,9 @@ def _lib():
         L.gmd_gemm_launch_mx.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                          C.c_void_p]
         L.gmd_mx_pack_scales.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]
+        L.gmd_block_quantize_launch.argtypes = [C.POINTER(BlockQuantize), C.c_void_p]
+        L.gmd_gemm_block_launch.argtypes = [C.POINTER(GemmBlock), C.c_void_p]
+        L.gmd_grouped_gemm_launch.argtypes = [C.POINTER(GroupedGemm), C.c_void_p]
         _typed = True
     return L
 
@@ -531,3 +534,63 @@ def mx_pack_scales(src_ptr, dst_ptr, rows, k, stream=None):
     rc = _lib().gmd_mx_pack_scales(C.c_void_p(src_ptr), C.c_void_p(dst_ptr), rows, k, C.c_void_p(stream))
     if rc:
         raise DiagError(rc, "gmd_mx_pack_scales")
+
+
+BLOCKS = {"rows": 0, "tiles": 1}
+GROUPED_OPS = {"forward": 0, "dgrad": 1, "wgrad": 2}
+
+
+class BlockQuantize(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("scales", C.c_void_p), ("ld_src", C.c_int64),
+                ("ld_dst", C.c_int64), ("ld_scales", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32),
+                ("src_dtype", C.c_int32), ("blocks", C.c_int32), ("transpose", C.c_int32), ("reserved", C.c_int32)]
+
+
+class GemmBlock(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("c", C.c_void_p), ("scale_a", C.c_void_p),
+                ("scale_b", C.c_void_p), ("lda", C.c_int64), ("ldb", C.c_int64), ("ldc", C.c_int64),
+                ("ld_scale_a", C.c_int64), ("ld_scale_b", C.c_int64), ("m", C.c_int32), ("n", C.c_int32),
+                ("k", C.c_int32), ("b_blocks", C.c_int32), ("out_dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class GroupedGemm(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("c", C.c_void_p), ("offsets", C.c_void_p),
+                ("scale_a", C.c_void_p), ("scale_b", C.c_void_p), ("lda", C.c_int64), ("ldb", C.c_int64),
+                ("ldc", C.c_int64), ("stride_w", C.c_int64), ("ld_scale_a", C.c_int64), ("ld_scale_b", C.c_int64),
+                ("stride_scale", C.c_int64), ("op", C.c_int32), ("dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("groups", C.c_int32), ("rows", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("reserved", C.c_int32)]
+
+
+def block_quantize_launch(src, dst, scales, rows, cols, dtype="bf16", blocks="rows", transpose=False, ld_src=0, ld_dst=0,
+                          ld_scales=0, stream=None):
+    """src [rows, cols] ("bf16" or "f32"), or src^T with `transpose`, -> e4m3 with one f32 scale per block of 128:
+    blocks="rows" (128 elements of a row; scales[ceil(c / 128)][r]) or "tiles" (128 x 128; scales[ceil(r / 128)][ceil(c / 128)]).
+    scale = amax / 448 with amax at least 2^-96; rows of dst are padded to a multiple of 16 with zeros.  Device pointers as
+    ints; strides in elements, 0 = packed."""
+    q = BlockQuantize(src, dst, scales, ld_src, ld_dst, ld_scales, rows, cols, DTYPES[dtype], BLOCKS[blocks], bool(transpose))
+    rc = _lib().gmd_block_quantize_launch(C.byref(q), stream)
+    if rc:
+        raise DiagError(rc, "gmd_block_quantize_launch")
+
+
+def gemm_block_launch(a, scale_a, b, scale_b, c, m, n, k, b_blocks="tiles", out="bf16", lda=0, ldb=0, ldc=0, ld_scale_a=0,
+                      ld_scale_b=0, stream=None):
+    """C[m, n] ("bf16" or "f32") = A[m, k] @ B[n, k]^T of e4m3 operands with an f32 scale per block of 128
+    (block_quantize_launch): A's blocks are rows, B's tiles or rows.  Any m, n a multiple of 8, k of 16."""
+    g = GemmBlock(a, b, c, scale_a, scale_b, lda, ldb, ldc, ld_scale_a, ld_scale_b, m, n, k, BLOCKS[b_blocks], DTYPES[out])
+    rc = _lib().gmd_gemm_block_launch(C.byref(g), stream)
+    if rc:
+        raise DiagError(rc, "gmd_gemm_block_launch")
+
+
+def grouped_gemm_launch(op, dtype, a, b, c, offsets, groups, rows, n, k, out="bf16", scale_a=None, scale_b=None, lda=0, ldb=0,
+                        ldc=0, stride_w=0, ld_scale_a=0, ld_scale_b=0, stride_scale=0, stream=None):
+    """One product per expert, rows sorted by expert: expert e owns rows offsets[e] .. offsets[e + 1] - 1 (int32 on the device).
+    "forward": c[rows, n] = a[rows, k] w[e]^T with b = w [groups][n, k]; "dgrad": c[rows, k] = a[rows, n] w[e];
+    "wgrad": c[groups][n, k] = per expert a[rows, n]^T b[rows, k].  dtype "bf16", or "fp8" (forward; e4m3 in blocks of
+    128 with scale_a per row and scale_b per tile of w).  Rows outside every expert's range are left as they were."""
+    g = GroupedGemm(a, b, c, offsets, scale_a, scale_b, lda, ldb, ldc, stride_w, ld_scale_a, ld_scale_b, stride_scale,
+                    GROUPED_OPS[op], DTYPES[dtype], DTYPES[out], groups, rows, n, k)
+    rc = _lib().gmd_grouped_gemm_launch(C.byref(g), stream)
+    if rc:
+        raise DiagError(rc, f"gmd_grouped_gemm_launch({op}, {dtype})")
