@@ -178,7 +178,8 @@ struct Stage {
   }
   // K-step kt into `tile`; `left` = k (elements if transposed, bytes if not) from this step on: what lies beyond is zero.
   __device__ __forceinline__ void fetch(int kt, int64_t left, char* tile, int wave) const {
-    const char* const src = base + (TRANS ? (int64_t)kt * 64 * ld : (int64_t)kt * kStepBytes);
+    const char* src = base + (TRANS ? (int64_t)kt * 64 * ld : (int64_t)kt * kStepBytes);
+    asm volatile("" : "+s"(src));  // one scalar base per step; otherwise the compiler keeps a 64-bit address per piece and lane
     char* const dst = tile + wave * kPieces * 1024;
     if (left >= (TRANS ? 64 : kStepBytes)) {
 #pragma unroll
@@ -247,27 +248,36 @@ __device__ __forceinline__ void widen(const i32x4& v, i32x4* lo, i32x4* hi) {
     (*to)[2 * (i & 1) + 1] = y;
   }
 }
-// What one K-step's fragment of e4m3 is multiplied as.  NARROW: on the K = 128 fp8 instruction.  That instruction aligns the
+// One K-step's fragment of an operand, by what it is multiplied as.  0: bf16.  1: e4m3 on the K = 128 fp8 instruction.  That instruction aligns the
 // products of each group of eight k to the largest of them and drops what lies below 2^-13 of its binade (measured with one large and one small product
 // per group; the K = 32 and K = 64 fp8 forms do the same), at most 2^-10 of the sum of
 // magnitudes and about 5e-6 of the result on normal data.  A bf16 result rounds coarser than that; an f32 result does not,
-// so for it the elements are widened to bf16 and multiplied on the bf16 instruction, which keeps f32 sums, at half the rate.
-template <bool NARROW>
-struct Wide;
+// so for it (2) the elements are widened to bf16 and multiplied on the bf16 instruction, which keeps f32 sums, at half the rate.
+template <int FORM>
+struct Operand;
 template <>
-struct Wide<true> {
-  i32x8 v;
-  __device__ __forceinline__ void set(const i32x4& lo, const i32x4& hi) { v = i32x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}; }
-  static __device__ __forceinline__ f32x4 product(const Wide& b, const Wide& a) { return mfma_fp8(b.v, a.v); }
+struct Operand<0> {
+  i32x4 v[2];
+  __device__ __forceinline__ void set(const i32x4& lo, const i32x4& hi) { v[0] = lo, v[1] = hi; }
+  static __device__ __forceinline__ void accumulate(const Operand& b, const Operand& a, f32x4& c) {
+    c = mfma_bf16(b.v[0], a.v[0], c);
+    c = mfma_bf16(b.v[1], a.v[1], c);
+  }
 };
 template <>
-struct Wide<false> {
+struct Operand<1> {
+  i32x8 v;
+  __device__ __forceinline__ void set(const i32x4& lo, const i32x4& hi) { v = i32x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}; }
+  static __device__ __forceinline__ f32x4 product(const Operand& b, const Operand& a) { return mfma_fp8(b.v, a.v); }
+};
+template <>
+struct Operand<2> {
   i32x4 v[4];
   __device__ __forceinline__ void set(const i32x4& lo, const i32x4& hi) {
     widen(lo, &v[0], &v[1]);
     widen(hi, &v[2], &v[3]);
   }
-  static __device__ __forceinline__ f32x4 product(const Wide& b, const Wide& a) {
+  static __device__ __forceinline__ f32x4 product(const Operand& b, const Operand& a) {
     f32x4 c{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; i++) c = mfma_bf16(b.v[i], a.v[i], c);
@@ -308,7 +318,9 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   constexpr int kABytes = BM * kStepBytes, kBufBytes = (BM + BN) * kStepBytes;
   constexpr int kStrip = WTN * 4 + 16;  // epilogue: one row of a wave's strip of 16 rows
   static_assert(kWaves * 16 * kStrip <= 2 * kBufBytes, "the epilogue's strips fit into the operand buffers");
-  __shared__ __attribute__((aligned(16))) char smem[2 * kBufBytes];
+  constexpr int kScaleWaves = kFp8 ? BM / 64 + (KIND == kFp8Rows ? BN / 64 : 1) : 0, kScaleBytes = kScaleWaves * 256;
+  static_assert(kScaleWaves <= kWaves && BN <= 64 * 128, "one DMA of scales per wave and step");
+  __shared__ __attribute__((aligned(16))) char smem[2 * kBufBytes + 2 * kScaleBytes];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -344,25 +356,44 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
 #pragma unroll
     for (int j = 0; j < NB; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // Scales of one K-step.
-  const int row0 = t.m0 + wm * WTM + fr * MB;  // the first of this lane's rows
-  const bool rows_whole = t.m0 + BM <= t.m_end;
+  // Scales of one K-step travel with its operands: A's of the tile's rows and B's of its columns (or of its 128-column
+  // tiles) in a slot of their own behind the operand buffers, one DMA of 4 bytes a lane for 64 of them.  Loaded by each wave for
+  // itself into registers they cost more than the matrix work: nine loads of their own per lane, wave and step.
   const float* const SB = kFp8 ? p.sb + t.group * p.stride_sb : nullptr;
-  float sa[MB], sa_next[MB];
-  f32x4 sb[NB], sb_next[NB];
-  auto load_scales = [&](int kt, float (&s)[MB], f32x4 (&u)[NB]) {
-    const float* q = p.sa + kt * p.ld_sa;
+  const float* scale_src = nullptr;  // this lane's, at step 0
+  int64_t scale_ld = 0;
+  if constexpr (kFp8) {
+    if (wave < BM / 64) {
+      scale_src = p.sa + min(t.m0 + wave * 64 + lane, t.m_end - 1), scale_ld = p.ld_sa;
+    } else if (KIND == kFp8Rows) {
+      scale_src = SB + min(t.n0 + (wave - BM / 64) * 64 + lane, p.n - 1), scale_ld = p.ld_sb;
+    } else {
+      scale_src = SB + (int64_t)(min(t.n0 + lane * 128, p.n - 1) / 128) * p.ld_sb, scale_ld = 1;
+    }
+  }
+  auto fetch_scales = [&](int kt) {
+    if (wave < kScaleWaves)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(scale_src + kt * scale_ld),
+                                       (__attribute__((address_space(3))) void*)(smem + 2 * kBufBytes + (kt & 1) * kScaleBytes + wave * 256), 4, 0, 0);
+  };
+  constexpr int kSb = KIND == kFp8Rows ? NB : 1;
+  float sl[MB];   // sa * sb (tiles) or sa (rows) of the running step
+  f32x4 sb[kSb];  // rows: sb of this lane's columns
+  auto read_scales = [&](int kt) {
+    const float* const q = (const float*)(smem + 2 * kBufBytes + (kt & 1) * kScaleBytes);
 #pragma unroll
-    for (int i = 0; i < MB; i++) s[i] = q[rows_whole ? row0 + i : min(row0 + i, t.m_end - 1)];
+    for (int i = 0; i < MB; i += 4) {
+      const f32x4 v = *(const f32x4*)(q + wm * WTM + fr * MB + i);
+#pragma unroll
+      for (int r = 0; r < 4; r++) sl[i + r] = v[r];
+    }
     if constexpr (KIND == kFp8Tiles) {
-      u[0][0] = SB[(int64_t)(min(t.n0 + wn * WTN, p.n - 1) / 128) * p.ld_sb + kt];  // (a wave's columns may all lie behind the last)
+      const float b = q[BM + wn * WTN / 128];
+#pragma unroll
+      for (int i = 0; i < MB; i++) sl[i] *= b;
     } else {
 #pragma unroll
-      for (int j = 0; j < NB; j++) {
-        const int col = min(t.n0 + wn * WTN + j * 16 + fq * 4, p.n - 4);
-        const float* r = SB + kt * p.ld_sb + col;
-        u[j] = f32x4{r[0], r[1], r[2], r[3]};
-      }
+      for (int j = 0; j < NB; j++) sb[j] = *(const f32x4*)(q + BM + wn * WTN + j * 16 + fq * 4);
     }
   };
 
@@ -372,54 +403,73 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
     const int64_t left = (int64_t)K - (int64_t)kt * kStepK;
     ga.fetch(kt, TA ? left : left * kElem, buf, wave);
     gb.fetch(kt, TB ? left : left * kElem, buf + kABytes, wave);
+    if constexpr (kFp8) fetch_scales(kt);
+  };
+
+  // One step: row blocks i = 0 .. MB-1 of the wave's tile against its NB column blocks.  A's fragment of the next row block
+  // is read while this one is multiplied.  The last row block holds the step's one synchronisation: every fragment of this
+  // buffer has been read and the next buffer has landed; behind it go the DMA of step kt + 2 into this buffer and the reads of
+  // the next step's first fragments, each of B's as soon as its registers have been consumed, so that the matrix pipe does not
+  // drain at a step's edge.
+  typedef Operand<kFp8 ? (kNarrow ? 1 : 2) : 0> Op;
+  Op bf[NB], af[2];
+  f32x4 part[4];       // block sums on their way to the accumulators
+  auto add = [&](int i, int j, int slot, float s) {
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+      acc[i][j][r] = __builtin_fmaf(KIND == kFp8Tiles ? s : s * sb[KIND == kFp8Tiles ? 0 : j][r], part[slot][r], acc[i][j][r]);
+    asm volatile("" : "+v"(acc[i][j]));  // here, between the MFMAs: left to itself the compiler sinks all of them behind the last
+  };
+  auto sync = [&]() {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0), as the builtin, so that the compiler's own count agrees
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
   if (steps > 0) {
-    if constexpr (kFp8) load_scales(0, sa, sb);
     fetch(0);
-    __syncthreads();  // waits for the LDS-DMA as well
+    if (steps > 1) fetch(1);
+    sync();
+    if constexpr (kFp8) read_scales(0);
+#pragma unroll
+    for (int j = 0; j < NB; j++) bf[j].set(fb.read(smem + kABytes, j, 0), fb.read(smem + kABytes, j, 1));
+    af[0].set(fa.read(smem, 0, 0), fa.read(smem, 0, 1));
   }
   for (int kt = 0; kt < steps; kt++) {
-    if (kt + 1 < steps) {
-      if constexpr (kFp8) load_scales(kt + 1, sa_next, sb_next);
-      fetch(kt + 1);
-    }
     const char* const la = smem + (kt & 1) * kBufBytes;
-    const char* const lb = la + kABytes;
-    if constexpr (kFp8) {
-      Wide<kNarrow> bf[NB], af;
+    const char* const na = smem + ((kt + 1) & 1) * kBufBytes;
+    const char* const nb = na + kABytes;
 #pragma unroll
-      for (int j = 0; j < NB; j++) bf[j].set(fb.read(lb, j, 0), fb.read(lb, j, 1));
-#pragma unroll
-      for (int i = 0; i < MB; i++) {
-        af.set(fa.read(la, i, 0), fa.read(la, i, 1));
-        const float s = KIND == kFp8Tiles ? sa[i] * sb[0][0] : sa[i];
-#pragma unroll
-        for (int j = 0; j < NB; j++) {
-          const f32x4 part = Wide<kNarrow>::product(bf[j], af);
-#pragma unroll
-          for (int r = 0; r < 4; r++) acc[i][j][r] = __builtin_fmaf(KIND == kFp8Tiles ? s : s * sb[j][r], part[r], acc[i][j][r]);
-        }
+    for (int i = 0; i < MB; i++) {
+      if (i + 1 < MB) {
+        af[(i + 1) & 1].set(fa.read(la, i + 1, 0), fa.read(la, i + 1, 1));
+      } else {
+        sync();
+        if (kt + 2 < steps) fetch(kt + 2);
+        af[0].set(fa.read(na, 0, 0), fa.read(na, 0, 1));  // (behind the last step: landed data that nothing uses)
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < MB; i++) sa[i] = sa_next[i];
-#pragma unroll
-      for (int j = 0; j < NB; j++) sb[j] = sb_next[j];
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        i32x4 bf[NB];
-#pragma unroll
-        for (int j = 0; j < NB; j++) bf[j] = fb.read(lb, j, h);
-#pragma unroll
-        for (int i = 0; i < MB; i++) {
-          const i32x4 af = fa.read(la, i, h);
-#pragma unroll
-          for (int j = 0; j < NB; j++) acc[i][j] = mfma_bf16(bf[j], af, acc[i][j]);
+      for (int j = 0; j < NB; j++) {
+        const int at = i * NB + j;
+        if constexpr (kFp8) {
+          part[at & 3] = Op::product(bf[j], af[i & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (at >= 2) add((at - 2) / NB, (at - 2) % NB, (at - 2) & 3, sl[(at - 2) / NB]);
+        } else {
+          Op::accumulate(bf[j], af[i & 1], acc[i][j]);
         }
+        if (i + 1 == MB) bf[j].set(fb.read(nb, j, 0), fb.read(nb, j, 1));
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    __syncthreads();  // the next buffer has landed and everyone is done with this one
+    if constexpr (kFp8) {
+      add(MB - 1, NB - 2, (MB * NB - 2) & 3, sl[MB - 1]);
+      add(MB - 1, NB - 1, (MB * NB - 1) & 3, sl[MB - 1]);
+      read_scales(kt + 1);
+    }
   }
+  __syncthreads();  // every wave is done with the operand buffers
 
   // Epilogue: 16 rows of the wave's tile at a time through a strip of LDS of its own, so that neighbouring lanes store
   // neighbouring columns of one row.
@@ -508,14 +558,14 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(Args p) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
       if (k0 + u * kFewWaves >= steps) break;
-      Wide<kNarrow> bf;
+      Operand<kNarrow ? 1 : 2> bf;
       if constexpr (kFp8) bf.set(bl[u], bh[u]);
 #pragma unroll
       for (int i = 0; i < MB; i++) {
         if constexpr (kFp8) {
-          Wide<kNarrow> af;
+          Operand<kNarrow ? 1 : 2> af;
           af.set(al[u][i], ah[u][i]);
-          const f32x4 part = Wide<kNarrow>::product(bf, af);
+          const f32x4 part = Operand<kNarrow ? 1 : 2>::product(bf, af);
 #pragma unroll
           for (int r = 0; r < 4; r++) acc[i][r] = __builtin_fmaf(sa[u][i] * (KIND == kFp8Tiles ? sb[u][0] : sb[u][r]), part[r], acc[i][r]);
         } else {
