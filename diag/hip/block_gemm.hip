@@ -78,7 +78,7 @@ int gmd_gemm_block_launch(const gmd_gemm_block_t* g, void* hip_stream) {
     bad = bad_operand(g->a, p.lda, g->k);
     if (!bad) bad = bad_operand(g->b, p.ldb, g->k);
     if (!bad && (!p.sa || !p.sb || (((uintptr_t)p.sa | (uintptr_t)p.sb) & 3))) bad = "null or misaligned scales";
-    if (!bad && (p.ld_sa < g->m || p.ld_sb < (g->b_blocks == GMD_BLOCK_TILES ? kb : g->n))) bad = "a stride of scales shorter than what it spans";
+    if (!bad && (p.ld_sa < g->m || p.ld_sb > 1 << 28 || p.ld_sb < (g->b_blocks == GMD_BLOCK_TILES ? kb : g->n))) bad = "a stride of scales shorter than what it spans, or over 2^28";
   }
   if (bad) {
     gmd::set_error("block GEMM: %s", bad);

@@ -7,6 +7,8 @@
 // A K-step is 128 bytes of k: 64 bf16 or one block of 128 e4m3.
 #pragma once
 
+#include <type_traits>
+
 #include "diag_common.h"
 
 namespace gmd {
@@ -52,10 +54,10 @@ __device__ __forceinline__ int xcd_contiguous(int id, int n) {
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
 }
 
-// Tiles in panels of eight rows of tiles, rows first inside a panel: neighbours share the B panel, and eight A panels
+// Tiles in panels of four rows of tiles, rows first inside a panel: neighbours share the B panel, and four A panels
 // are walked again for the next column.
 __device__ __forceinline__ void tile_walk(int id, int tiles_m, int tiles_n, int* tm, int* tn) {
-  const int panel = id / (8 * tiles_n), first = panel * 8, rows = min(8, tiles_m - first), in = id - panel * 8 * tiles_n;
+  const int panel = id / (4 * tiles_n), first = panel * 4, rows = min(4, tiles_m - first), in = id - panel * 4 * tiles_n;
   *tm = first + in % rows;
   *tn = in / rows;
 }
@@ -133,80 +135,102 @@ __device__ __forceinline__ int chunk_swizzle(int row) { return ((row >> 1) & 3) 
 
 // Transposed: 64 rows of k, the m or n side contiguous.  Fragments come through ds_read_b64_tr_b16: within each group of 16
 // lanes lane i supplies the address of 4 elements of row i / 4, columns 4 (i % 4) .., and receives column i of the four rows.
-// A read's 16 rows are a multiple of the row size apart, so 32-byte units of a row are permuted by unit ^ f(row) with f
-// running over all eight values within the rows that half a wave touches.
-__device__ __forceinline__ int unit_swizzle(int row) { return ((row >> 3) & 1) * 4 + (row & 3); }
-
-__device__ __forceinline__ void load_lds16(const char* src, char* dst) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+// Half a wave touches rows 0-3 and 8-11 (and the like), 32 bytes each; the 32-byte units of a row are permuted by
+// unit ^ unit_swizzle(row) so that these eight units lie in different banks (64 banks of 4 bytes).  COLS: columns of the image.
+template <int COLS>
+__device__ __forceinline__ int unit_swizzle(int row) {
+  if constexpr (COLS >= 128) return ((row >> 3) & 1) * 4 + (row & 3);
+  if constexpr (COLS == 64) return ((row >> 3) & 1) * 2 + ((row >> 1) & 1);
+  return (row >> 3) & 1;
 }
 
-// One operand's way into LDS.  ROWS: rows of the tile (its m or n extent); WAVES share the 1-KiB pieces.  DEAL: LDS row
-// 16 b + f of a wave's WT rows holds tile row f * (WT / 16) + b, so that a fragment lane's rows are consecutive.
-template <bool TRANS, int ROWS, int WAVES, int DEAL>
+// One LDS-DMA instruction: SGPR base + 32-bit VGPR offset -> M0 + lane * BYTES.  Through the builtin every one costs a 64-bit
+// vector add as well, and the compiler keeps the addresses of a whole step in registers.
+template <int BYTES>
+__device__ __forceinline__ void dma(const void* src, uint32_t off, char* dst) {
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dst;
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(src), "s"(lds) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(src), "s"(lds) : "memory", "m0");
+}
+
+// One operand's way into LDS.  ROWS: rows of the tile (its m or n extent); WAVES share the 1-KiB pieces.
+// HALVES = the rows WT of a wave's tile: the first half of a wave's pieces fill the first half of every wave's rows, so that
+// the two halves can be fetched and waited for apart (transposed: an image of its own for each wave row and half); 0: no halves.
+// DEAL (k contiguous, halves): LDS row 16 b + f of a wave's rows holds row f * (WT / 16) + b, so that a fragment lane's rows are
+// consecutive.
+template <bool TRANS, int ROWS, int WAVES, int HALVES, bool DEAL>
 struct Stage {
   static constexpr int kPieces = ROWS / 8 / WAVES;
-  static_assert(kPieces * 8 * WAVES == ROWS, "whole pieces per wave");
-  static constexpr int kChunks = ROWS / 8;  // transposed: 16-byte chunks per row of k
+  static_assert(kPieces * 8 * WAVES == ROWS && (!HALVES || kPieces % 2 == 0), "whole pieces per wave and half");
+  static constexpr int kCols = HALVES ? HALVES / 2 : ROWS;  // transposed: columns of an image
+  static constexpr int kChunks = kCols / 8;                 // ... and 16-byte chunks of its rows, which is also its size in KiB
   const char* base;        // first row of the tile, first k
   uint32_t off[kPieces];   // a lane's place in it
   int chunk[kPieces];      // its chunk of the 128 bytes (k contiguous) or its row of the 64 (transposed)
   int64_t ld;
 
+  // Which KiB of the tile's image piece i of a wave is.
+  static __device__ __forceinline__ int place(int wave, int i) {
+    if constexpr (HALVES == 0) return wave * kPieces + i;
+    constexpr int per = kPieces / 2, block = HALVES / 16;  // pieces per wave and half; KiB of one wave row's half
+    const int q = wave * per + i % per;                    // among the pieces of this half
+    return q / block * 2 * block + i / per * block + q % block;
+  }
   // first: first row (column) of the tile, rows_left >= 1: how many of them exist; the rest repeat the last one.
   __device__ __forceinline__ void init(const char* p, int64_t ld_, int64_t first, int rows_left, int wave, int lane) {
     ld = ld_;
     base = TRANS ? p + first * 2 : p + first * ld;
 #pragma unroll
     for (int i = 0; i < kPieces; i++) {
-      const int piece = wave * kPieces + i;
+      const int piece = place(wave, i);
       if constexpr (TRANS) {
-        const int pos = piece * 64 + lane, r = pos / kChunks;
-        const int c = (pos % kChunks) ^ ((2 * unit_swizzle(r)) & (kChunks - 1));
-        const int col = min(c * 8, rows_left - 8);  // the extent is a multiple of 8
+        const int image = piece / kChunks, pos = piece % kChunks * 64 + lane, r = pos / kChunks;
+        const int c = (pos % kChunks) ^ (2 * unit_swizzle<kCols>(r));
+        const int col = min(image * kCols + c * 8, rows_left - 8);  // the extent is a multiple of 8
         off[i] = (uint32_t)(r * ld) + (uint32_t)col * 2;
         chunk[i] = r;
       } else {
         const int l = piece * 8 + (lane >> 3);
         int row = l;
-        if constexpr (DEAL != 0) row = l / DEAL * DEAL + (l & 15) * (DEAL / 16) + (l % DEAL >> 4);
+        if constexpr (DEAL) row = l / HALVES * HALVES + (l & 15) * (HALVES / 16) + (l % HALVES >> 4);
         const int c = (lane & 7) ^ chunk_swizzle(l);
         off[i] = (uint32_t)(min(row, rows_left - 1) * ld) + (uint32_t)c * 16;
         chunk[i] = c;
       }
     }
   }
-  // K-step kt into `tile`; `left` = k (elements if transposed, bytes if not) from this step on: what lies beyond is zero.
-  __device__ __forceinline__ void fetch(int kt, int64_t left, char* tile, int wave) const {
-    const char* src = base + (TRANS ? (int64_t)kt * 64 * ld : (int64_t)kt * kStepBytes);
-    asm volatile("" : "+s"(src));  // one scalar base per step; otherwise the compiler keeps a 64-bit address per piece and lane
-    char* const dst = tile + wave * kPieces * 1024;
-    if (left >= (TRANS ? 64 : kStepBytes)) {
-#pragma unroll
-      for (int i = 0; i < kPieces; i++) load_lds16(src + off[i], dst + i * 1024);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPieces; i++) {
-        const bool in = TRANS ? chunk[i] < left : chunk[i] * 16 < left;
-        load_lds16(in ? src + off[i] : (const char*)&g_zero16, dst + i * 1024);
-      }
-    }
+  __device__ __forceinline__ const char* step_base(int kt) const {
+    return base + (TRANS ? (int64_t)kt * 64 * ld : (int64_t)kt * kStepBytes);
+  }
+  // Piece i of a K-step that lies inside k as a whole.
+  __device__ __forceinline__ void fetch(const char* src, char* tile, int wave, int i) const {
+    dma<16>(src, off[i], tile + place(wave, i) * 1024);
+  }
+  // Piece i of any K-step; `left` = k (elements if transposed, bytes if not) from this step on: what lies beyond is zero.
+  __device__ __forceinline__ void fetch_edge(const char* src, int64_t left, char* tile, int wave, int i) const {
+    const bool in = TRANS ? chunk[i] < left : chunk[i] * 16 < left;
+    const char* const from = in ? src + off[i] : (const char*)&g_zero16;
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)(tile + place(wave, i) * 1024), 16, 0, 0);
   }
 };
 
 // A wave's fragments of one operand: blocks of 16 rows, two halves of the K-step each (bf16: two substeps of 32 k; fp8:
 // registers 0-3 and 4-7 of the one K = 128 operand).
-template <bool TRANS, int ROWS, int NB>
+template <bool TRANS, int ROWS, int NB, int HALVES>
 struct Frags {
+  static constexpr int kCols = HALVES ? HALVES / 2 : ROWS;
   int off[TRANS ? NB : 2];
   __device__ __forceinline__ void init(int first, int lane) {
     const int fr = lane & 15, fq = lane >> 4;
     if constexpr (TRANS) {
-      const int r = 8 * fq + (fr >> 2);
+      const int r = 8 * fq + (fr >> 2);  // (rows 4, 32 and 36 further on have the same permutation)
 #pragma unroll
       for (int b = 0; b < NB; b++) {
-        const int unit = (first / 16 + b) ^ (unit_swizzle(r) & (ROWS / 16 - 1));
-        off[b] = r * (ROWS * 2) + unit * 32 + (fr & 3) * 8;
+        const int col = first + 16 * b;
+        off[b] = col / kCols * (kCols * 128) + r * (kCols * 2) + ((col % kCols / 16) ^ unit_swizzle<kCols>(r)) * 32 + (fr & 3) * 8;
       }
     } else {
       const int l = first + fr;
@@ -219,9 +243,9 @@ struct Frags {
       typedef short s16x4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
       typedef int i32x2 __attribute__((ext_vector_type(2)));
-      const char* q = tile + off[b] + h * 32 * (ROWS * 2);
+      const char* q = tile + off[b] + h * 32 * (kCols * 2);
       const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)q));
-      const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 4 * (ROWS * 2))));
+      const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(q + 4 * (kCols * 2))));
       return i32x4{lo.x, lo.y, hi.x, hi.y};
     } else {
       return *(const i32x4*)(tile + off[h] + b * 2048);
@@ -318,8 +342,8 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   constexpr int kABytes = BM * kStepBytes, kBufBytes = (BM + BN) * kStepBytes;
   constexpr int kStrip = WTN * 4 + 16;  // epilogue: one row of a wave's strip of 16 rows
   static_assert(kWaves * 16 * kStrip <= 2 * kBufBytes, "the epilogue's strips fit into the operand buffers");
-  constexpr int kScaleWaves = kFp8 ? BM / 64 + (KIND == kFp8Rows ? BN / 64 : 1) : 0, kScaleBytes = kScaleWaves * 256;
-  static_assert(kScaleWaves <= kWaves && BN <= 64 * 128, "one DMA of scales per wave and step");
+  constexpr int kScaleBytes = kFp8 ? kWaves * 256 : 0;
+  static_assert(BM / 64 + (KIND == kFp8Rows ? BN / 64 : 1) <= kWaves, "one DMA of scales per wave and step");
   __shared__ __attribute__((aligned(16))) char smem[2 * kBufBytes + 2 * kScaleBytes];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -341,12 +365,14 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
     if (!find_tile(p, BM, BN, blockIdx.x, &t)) return;  // the whole workgroup, before any barrier
   }
   const char* const B = p.b + (WGRAD ? 0 : t.group * p.stride_b);
-  Stage<TA, BM, kWaves, kFp8 ? WTM : 0> ga;
-  Stage<TB, BN, kWaves, 0> gb;
+  typedef Stage<TA, BM, kWaves, WTM, kFp8> StageA;
+  typedef Stage<TB, BN, kWaves, 0, false> StageB;
+  StageA ga;
+  StageB gb;
   ga.init(p.a + (TA ? k_first * p.lda : 0), p.lda, t.m0, t.m_end - t.m0, wave, lane);
   gb.init(B + (TB ? k_first * p.ldb : 0), p.ldb, t.n0, p.n - t.n0, wave, lane);
-  Frags<TA, BM, MB> fa;
-  Frags<TB, BN, NB> fb;
+  Frags<TA, BM, MB, WTM> fa;
+  Frags<TB, BN, NB, 0> fb;
   fa.init(wm * WTM, lane);
   fb.init(wn * WTN, lane);
 
@@ -360,21 +386,25 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   // tiles) in a slot of their own behind the operand buffers, one DMA of 4 bytes a lane for 64 of them.  Loaded by each wave for
   // itself into registers they cost more than the matrix work: nine loads of their own per lane, wave and step.
   const float* const SB = kFp8 ? p.sb + t.group * p.stride_sb : nullptr;
-  const float* scale_src = nullptr;  // this lane's, at step 0
+  const float* scale_src = nullptr;  // at step 0, this wave's part
+  uint32_t scale_off = 0;            // this lane's place in it
   int64_t scale_ld = 0;
   if constexpr (kFp8) {
     if (wave < BM / 64) {
-      scale_src = p.sa + min(t.m0 + wave * 64 + lane, t.m_end - 1), scale_ld = p.ld_sa;
+      const int row = t.m0 + wave * 64;
+      scale_src = p.sa + min(row, t.m_end - 1), scale_ld = p.ld_sa;
+      scale_off = (uint32_t)max(min(lane, t.m_end - 1 - row), 0) * 4;
     } else if (KIND == kFp8Rows) {
-      scale_src = SB + min(t.n0 + (wave - BM / 64) * 64 + lane, p.n - 1), scale_ld = p.ld_sb;
-    } else {
-      scale_src = SB + (int64_t)(min(t.n0 + lane * 128, p.n - 1) / 128) * p.ld_sb, scale_ld = 1;
+      const int col = t.n0 + (wave - BM / 64) * 64;
+      scale_src = SB + min(col, p.n - 1), scale_ld = p.ld_sb;
+      scale_off = (uint32_t)max(min(lane, p.n - 1 - col), 0) * 4;
+    } else {  // (all waves that are left, so that every wave has as many DMAs in flight)
+      scale_src = SB + (int64_t)(t.n0 / 128) * p.ld_sb, scale_ld = 1;
+      scale_off = (uint32_t)(min(min(lane, BN / 128 - 1), (p.n - 1) / 128 - t.n0 / 128) * p.ld_sb * 4);
     }
   }
   auto fetch_scales = [&](int kt) {
-    if (wave < kScaleWaves)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(scale_src + kt * scale_ld),
-                                       (__attribute__((address_space(3))) void*)(smem + 2 * kBufBytes + (kt & 1) * kScaleBytes + wave * 256), 4, 0, 0);
+    dma<4>(scale_src + kt * scale_ld, scale_off, smem + 2 * kBufBytes + (kt & 1) * kScaleBytes + wave * 256);
   };
   constexpr int kSb = KIND == kFp8Rows ? NB : 1;
   float sl[MB];   // sa * sb (tiles) or sa (rows) of the running step
@@ -388,85 +418,164 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
       for (int r = 0; r < 4; r++) sl[i + r] = v[r];
     }
     if constexpr (KIND == kFp8Tiles) {
-      const float b = q[BM + wn * WTN / 128];
-#pragma unroll
-      for (int i = 0; i < MB; i++) sl[i] *= b;
+      sb[0][0] = q[BM + wn * WTN / 128];
     } else {
 #pragma unroll
       for (int j = 0; j < NB; j++) sb[j] = *(const f32x4*)(q + BM + wn * WTN + j * 16 + fq * 4);
     }
   };
+  auto join_scales = [&]() {  // tiles; apart from the reads, which it has to wait for
+#pragma unroll
+    for (int i = 0; i < MB; i++) sl[i] *= sb[0][0];
+  };
 
   const int steps = (int)(((int64_t)K + kStepK - 1) / kStepK);
-  auto fetch = [&](int kt) {
+  const int whole = K / kStepK;  // steps that lie inside k
+  // The DMAs of one step and wave in the order they are issued: B, the first half of A, the scales (the first kFirst), and
+  // the second half of A (kSecond).
+  constexpr int kHalfA = StageA::kPieces / 2, kFirst = StageB::kPieces + kHalfA + (kFp8 ? 1 : 0), kSecond = kHalfA;
+  auto fetch = [&](int kt, const char* src_a, const char* src_b, int piece) {
+    char* const buf = smem + (kt & 1) * kBufBytes;
+    if (piece < StageB::kPieces) gb.fetch(src_b, buf + kABytes, wave, piece);
+    else if (piece < StageB::kPieces + kHalfA) ga.fetch(src_a, buf, wave, piece - StageB::kPieces);
+    else if (kFp8 && piece == kFirst - 1) fetch_scales(kt);
+    else ga.fetch(src_a, buf, wave, piece - kFirst + kHalfA);
+  };
+  auto fetch_edge = [&](int kt, int from, int to) {
     char* const buf = smem + (kt & 1) * kBufBytes;
     const int64_t left = (int64_t)K - (int64_t)kt * kStepK;
-    ga.fetch(kt, TA ? left : left * kElem, buf, wave);
-    gb.fetch(kt, TB ? left : left * kElem, buf + kABytes, wave);
-    if constexpr (kFp8) fetch_scales(kt);
+#pragma unroll
+    for (int piece = from; piece < to; piece++) {
+      if (piece < StageB::kPieces) gb.fetch_edge(gb.step_base(kt), TB ? left : left * kElem, buf + kABytes, wave, piece);
+      else if (piece < StageB::kPieces + kHalfA) ga.fetch_edge(ga.step_base(kt), TA ? left : left * kElem, buf, wave, piece - StageB::kPieces);
+      else if (kFp8 && piece == kFirst - 1) fetch_scales(kt);
+      else ga.fetch_edge(ga.step_base(kt), TA ? left : left * kElem, buf, wave, piece - kFirst + kHalfA);
+    }
   };
 
-  // One step: row blocks i = 0 .. MB-1 of the wave's tile against its NB column blocks.  A's fragment of the next row block
-  // is read while this one is multiplied.  The last row block holds the step's one synchronisation: every fragment of this
-  // buffer has been read and the next buffer has landed; behind it go the DMA of step kt + 2 into this buffer and the reads of
-  // the next step's first fragments, each of B's as soon as its registers have been consumed, so that the matrix pipe does not
-  // drain at a step's edge.
+  // One step multiplies the wave's MB row blocks by its NB column blocks, row by row, A's fragment of the next row block being
+  // read meanwhile; B's stay in registers for the step.  The last two row blocks go in halves, (MB-2, first half) | (MB-1, first
+  // half) (MB-2, second half) (MB-1, second half), and behind the bar each of B's fragments of the next step is read as soon as
+  // its registers have been consumed, so that the matrix pipe does not drain at a step's edge.
+  // Two buffers, refilled in halves so that the DMA never drains either: two synchronisations per step,
+  //   kMid (the first half of A and all of B have been read): the second half of A must have landed; B, the first half of A and
+  //        the scales of step kt + 2 go out;
+  //   kBar (all of A has been read): B, the first half of A and the scales of step kt + 1 must have landed; the second half of A
+  //        of step kt + 2 goes out.
+  // Each has one and a half steps to arrive, with the other group in flight behind it (the counted waits).  With the whole
+  // buffer refilled at kBar and waited for a step later, a step could not be shorter than a memory latency plus its 64 KiB:
+  // 8192^3 block-scaled 505 us.
+  constexpr int kProducts = MB * NB, kTail = (MB - 2) * NB, kHalf = NB / 2, kBar = kTail + kHalf, kMid = (MB / 2 - 1) * NB;
+  constexpr int kPer = (kFirst + kBar - kMid - 1) / (kBar - kMid);  // DMAs behind one product, all of the first group before kBar
+  static_assert(MB >= 4 && MB % 2 == 0 && NB == 4 && kSecond <= kProducts - kBar, "the pieces fit behind the products");
+  auto row_of = [](int at) { return at < kTail ? at / NB : MB - 2 + (at - kTail) / kHalf % 2; };
+  auto col_of = [](int at) { return at < kTail ? at % NB : (at - kTail) % kHalf + (at - kTail >= NB ? kHalf : 0); };
   typedef Operand<kFp8 ? (kNarrow ? 1 : 2) : 0> Op;
   Op bf[NB], af[2];
-  f32x4 part[4];       // block sums on their way to the accumulators
-  auto add = [&](int i, int j, int slot, float s) {
+  f32x4 part[4];       // block sums on their way to the accumulators, two MFMAs behind
+  float s_tail[2];     // the scales of the last two row blocks, while the next step's arrive
+  auto add = [&](int at) {
+    const int i = row_of(at), j = col_of(at);
+    const float s = KIND == kFp8Rows || i < MB - 2 ? sl[i] : s_tail[i - (MB - 2)];
 #pragma unroll
     for (int r = 0; r < 4; r++)
-      acc[i][j][r] = __builtin_fmaf(KIND == kFp8Tiles ? s : s * sb[KIND == kFp8Tiles ? 0 : j][r], part[slot][r], acc[i][j][r]);
+      acc[i][j][r] = __builtin_fmaf(KIND == kFp8Tiles ? s : s * sb[KIND == kFp8Tiles ? 0 : j][r], part[at & 3][r], acc[i][j][r]);
     asm volatile("" : "+v"(acc[i][j]));  // here, between the MFMAs: left to itself the compiler sinks all of them behind the last
   };
-  auto sync = [&]() {
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0), as the builtin, so that the compiler's own count agrees
+  // vmcnt(behind) lgkmcnt(0) and a barrier; `behind`: DMAs that may stay in flight.
+  auto sync = [&](auto behind) {
+    constexpr int n = decltype(behind)::value;
+    __builtin_amdgcn_s_waitcnt((n & 15) | 0x70 | (n >> 4) << 14);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
+  const std::integral_constant<int, 0> none;
+  const std::integral_constant<int, kFirst + kSecond> step_behind;
+  const std::integral_constant<int, kSecond> second_behind;
   if (steps > 0) {
-    fetch(0);
-    if (steps > 1) fetch(1);
-    sync();
-    if constexpr (kFp8) read_scales(0);
+    fetch_edge(0, 0, kFirst + kSecond);
+    if (steps > 1) {
+      fetch_edge(1, 0, kFirst + kSecond);
+      sync(std::integral_constant<int, kFirst + 2 * kSecond>());
+    } else {
+      sync(second_behind);
+    }
 #pragma unroll
-    for (int j = 0; j < NB; j++) bf[j].set(fb.read(smem + kABytes, j, 0), fb.read(smem + kABytes, j, 1));
-    af[0].set(fa.read(smem, 0, 0), fa.read(smem, 0, 1));
+    for (int j = 0; j < NB; j++) {
+      bf[j].set(fb.read(smem + kABytes, j, 0), fb.read(smem + kABytes, j, 1));
+      if (j == kHalf - 1) af[0].set(fa.read(smem, 0, 0), fa.read(smem, 0, 1));
+    }
+    if constexpr (kFp8) {
+      read_scales(0);
+      if constexpr (KIND == kFp8Tiles) join_scales();
+#pragma unroll
+      for (int i = 0; i < 4; i++) part[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      s_tail[0] = s_tail[1] = 0.f;
+    }
   }
-  for (int kt = 0; kt < steps; kt++) {
+  // FULL: step kt + 2 exists and lies inside k.
+  auto step = [&](int kt, auto FULL) {
+    constexpr bool kFull = decltype(FULL)::value;
     const char* const la = smem + (kt & 1) * kBufBytes;
     const char* const na = smem + ((kt + 1) & 1) * kBufBytes;
     const char* const nb = na + kABytes;
+    const bool more = kFull || kt + 1 < steps, more2 = kFull || kt + 2 < steps;
+    const char* const src_a = ga.step_base(kt + 2);
+    const char* const src_b = gb.step_base(kt + 2);
 #pragma unroll
-    for (int i = 0; i < MB; i++) {
-      if (i + 1 < MB) {
-        af[(i + 1) & 1].set(fa.read(la, i + 1, 0), fa.read(la, i + 1, 1));
-      } else {
-        sync();
-        if (kt + 2 < steps) fetch(kt + 2);
-        af[0].set(fa.read(na, 0, 0), fa.read(na, 0, 1));  // (behind the last step: landed data that nothing uses)
+    for (int at = 0; at < kProducts; at++) {
+      const int i = row_of(at), j = col_of(at);
+      if (at == kMid) {
+        if (more) sync(step_behind);
+        else sync(none);
+        if (!kFull && more2) fetch_edge(kt + 2, 0, kFirst);
+      }
+      if (at % NB == 0 && at <= kTail) af[(i + 1) & 1].set(fa.read(la, i + 1, 0), fa.read(la, i + 1, 1));
+      if (at == kBar) {
+        if (more2) sync(step_behind);
+        else sync(none);
+        if (!kFull && more2) fetch_edge(kt + 2, kFirst, kFirst + kSecond);
+        if constexpr (KIND == kFp8Tiles) {
+          s_tail[0] = sl[MB - 2], s_tail[1] = sl[MB - 1];
+          read_scales(kt + 1);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int j = 0; j < NB; j++) {
-        const int at = i * NB + j;
-        if constexpr (kFp8) {
-          part[at & 3] = Op::product(bf[j], af[i & 1]);
-          __builtin_amdgcn_sched_barrier(0);
-          if (at >= 2) add((at - 2) / NB, (at - 2) % NB, (at - 2) & 3, sl[(at - 2) / NB]);
-        } else {
-          Op::accumulate(bf[j], af[i & 1], acc[i][j]);
-        }
-        if (i + 1 == MB) bf[j].set(fb.read(nb, j, 0), fb.read(nb, j, 1));
+      if constexpr (kFp8) {
+        part[at & 3] = Op::product(bf[j], af[i & 1]);
         __builtin_amdgcn_sched_barrier(0);
+        if (KIND == kFp8Tiles || at >= 2) add((at + kProducts - 2) % kProducts);  // (at first the last two of the step before, or zeros)
+      } else {
+        Op::accumulate(bf[j], af[i & 1], acc[i][j]);
       }
+      if (i == MB - 1) bf[j].set(fb.read(nb, j, 0), fb.read(nb, j, 1));  // (behind the last step: landed data that nothing uses)
+      if (at == kTail + NB + kHalf - 1) af[0].set(fa.read(na, 0, 0), fa.read(na, 0, 1));
+      if constexpr (kFull) {
+        if (at >= kMid && at < kBar) {
+#pragma unroll
+          for (int q = (at - kMid) * kPer; q < (at - kMid + 1) * kPer && q < kFirst; q++) fetch(kt + 2, src_a, src_b, q);
+        } else if (at >= kBar && at - kBar < kSecond) {
+          fetch(kt + 2, src_a, src_b, kFirst + at - kBar);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (kFp8) {
-      add(MB - 1, NB - 2, (MB * NB - 2) & 3, sl[MB - 1]);
-      add(MB - 1, NB - 1, (MB * NB - 1) & 3, sl[MB - 1]);
+    if constexpr (KIND == kFp8Tiles) {
+      join_scales();
+    } else if constexpr (kFp8) {  // no registers for a second set of B's scales: the last two sums are added first
+      add(kProducts - 2);
+      add(kProducts - 1);
       read_scales(kt + 1);
+    }
+  };
+  int kt = 0;
+  for (; kt + 2 < whole; kt++) step(kt, std::true_type());
+  for (; kt < steps; kt++) step(kt, std::false_type());
+  if constexpr (KIND == kFp8Tiles) {
+    if (steps > 0) {
+      add(kProducts - 2);
+      add(kProducts - 1);
     }
   }
   __syncthreads();  // every wave is done with the operand buffers

@@ -94,7 +94,7 @@ int gmd_grouped_gemm_launch(const gmd_grouped_gemm_t* g, void* hip_stream) {
     p.ld_sb = g->ld_scale_b ? g->ld_scale_b : kb;
     p.stride_sb = g->stride_scale ? g->stride_scale : nb * p.ld_sb;
     if (!p.sa || !p.sb || (((uintptr_t)p.sa | (uintptr_t)p.sb) & 3)) bad = "null or misaligned scales";
-    else if (p.ld_sa < g->rows || p.ld_sb < kb || p.stride_sb < (nb - 1) * p.ld_sb + kb) bad = "a stride of scales shorter than what it spans";
+    else if (p.ld_sa < g->rows || p.ld_sb > 1 << 28 || p.ld_sb < kb || p.stride_sb < (nb - 1) * p.ld_sb + kb) bad = "a stride of scales shorter than what it spans, or over 2^28";
   }
   if (bad) return refuse(bad);
   if (fp8) return launch_fp8(p, GMD_BLOCK_TILES, g->out_dtype, (hipStream_t)hip_stream);
