@@ -31,64 +31,108 @@ struct QuantArgs {
   int vec;                            // src rows can be read in 16-byte pieces
 };
 
-// A workgroup takes one 128 x 128 region of src into registers: thread t holds eight consecutive columns 8 (t % 16) of rows
-// t / 16 + 16 i.  That fits all four forms: a row's block lies in 16 neighbouring lanes, a column's in the 16 row groups of
-// four waves, a tile in the workgroup.
+// Eight consecutive elements of a row as f32; zeros outside the matrix.
+template <typename SRC>
+__device__ __forceinline__ void load8(const QuantArgs& p, int row, int col, float (&x)[8]) {
+  const SRC* s = (const SRC*)p.src + (int64_t)row * p.ld_src + col;
+  if (row < p.rows && p.vec && col + 8 <= p.cols) {
+    if constexpr (sizeof(SRC) == 2) {
+      const u32x4 v = *(const u32x4*)s;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        x[2 * j] = __builtin_bit_cast(float, v[j] << 16);
+        x[2 * j + 1] = __builtin_bit_cast(float, v[j] & 0xffff0000u);
+      }
+    } else {
+      const f32x4 v = *(const f32x4*)s, w = *(const f32x4*)(s + 4);
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[j] = v[j], x[4 + j] = w[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = row < p.rows && col + j < p.cols ? (float)s[j] : 0.f;
+  }
+}
+__device__ __forceinline__ unsigned magnitude8(const float (&x)[8]) {
+  unsigned m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) m = max(m, magnitude(x[j]));
+  return m;
+}
+__device__ __forceinline__ unsigned e4m3x4(float a, float b, float c, float d) {
+  const unsigned v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
+}
+
+// Blocks of a row, not transposed: a wave takes 512 columns (four blocks, sixteen lanes each) of eight rows, all loads in
+// flight before the first is used.  Memory-bound: reads of 1 KiB (bf16) and writes of 512 bytes per wave and row.
+constexpr int kRowsWave = 8, kRowsGroup = 32, kColsGroup = 512;
+template <typename SRC>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs p) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int groups_c = (p.cols + kColsGroup - 1) / kColsGroup;
+  const int row0 = (int)blockIdx.x / groups_c * kRowsGroup + wave * kRowsWave;
+  const int col = (int)blockIdx.x % groups_c * kColsGroup + lane * 8;
+  if (row0 >= p.rows) return;
+  float x[kRowsWave][8];
+#pragma unroll
+  for (int i = 0; i < kRowsWave; i++) load8<SRC>(p, row0 + i, col, x[i]);
+  const int last16 = (p.cols + 15) & ~15;
+  float scale[kRowsWave];
+#pragma unroll
+  for (int i = 0; i < kRowsWave; i++) {
+    unsigned m = magnitude8(x[i]);
+#pragma unroll
+    for (int off = 8; off; off >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, off, 16));
+    float inv;
+    scale_of(m, &scale[i], &inv);
+    // elements up to the next multiple of 16 columns are written, as zeros behind the last one
+    if (row0 + i < p.rows && col < last16)
+      *(u32x2*)(p.dst + (int64_t)(row0 + i) * p.ld_dst + col) = u32x2{e4m3x4(x[i][0] * inv, x[i][1] * inv, x[i][2] * inv, x[i][3] * inv),
+                                                                      e4m3x4(x[i][4] * inv, x[i][5] * inv, x[i][6] * inv, x[i][7] * inv)};
+  }
+  if ((lane & 15) == 0 && col < p.cols) {
+    float* const to = p.scales + (int64_t)(col / 128) * p.ld_scales + row0;
+    if (row0 + kRowsWave <= p.rows) {
+      __builtin_memcpy(to, scale, sizeof scale);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRowsWave; i++)
+        if (row0 + i < p.rows) to[i] = scale[i];
+    }
+  }
+}
+
+// The other three forms: a workgroup takes one 128 x 128 region of src into registers, thread t the eight consecutive columns
+// 8 (t % 16) of rows 4 (t / 16) + r + 64 h (r < 4, h < 2), so that a column's block lies in the sixteen row groups and a tile in the
+// workgroup, and four rows of a column pack into one dword of the transposed image.  In that image (128 bytes per column)
+// the 16-byte chunks of a column are permuted by chunk ^ (column / 8), which leaves the dword writes at two per bank and the
+// 16-byte reads at one.
 template <typename SRC, bool TILES, bool TRANS>
-__global__ __launch_bounds__(256) void quantize_kernel(QuantArgs p) {
-  constexpr int kRows = 8;
+__global__ __launch_bounds__(256) void quantize_region_kernel(QuantArgs p) {
+  static_assert(TILES || TRANS, "rows are quantize_rows_kernel's");
   const int t = threadIdx.x, c16 = t & 15, rg = t >> 4;
   const int regions_c = (p.cols + 127) / 128;
   const int br = blockIdx.x / regions_c, bc = blockIdx.x % regions_c;
   const int col = bc * 128 + c16 * 8;
-  __shared__ unsigned red[16][132];
-  __shared__ __attribute__((aligned(16))) uint8_t turned[TRANS ? 128 * 144 : 16];
+  __shared__ unsigned red[TILES ? 1 : 16][128];
+  __shared__ __attribute__((aligned(16))) unsigned turned[TRANS ? 128 * 32 : 4];
 
-  float x[kRows][8];
+  float x[2][4][8];
 #pragma unroll
-  for (int i = 0; i < kRows; i++) {
-    const int row = br * 128 + rg + 16 * i;
-    const SRC* s = (const SRC*)p.src + (int64_t)row * p.ld_src + col;
-    if (row < p.rows && p.vec && col + 8 <= p.cols) {
-      if constexpr (sizeof(SRC) == 2) {
-        const u32x4 v = *(const u32x4*)s;
+  for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          x[i][2 * j] = __builtin_bit_cast(float, v[j] << 16);
-          x[i][2 * j + 1] = __builtin_bit_cast(float, v[j] & 0xffff0000u);
-        }
-      } else {
-        const f32x4 v = *(const f32x4*)s, w = *(const f32x4*)(s + 4);
-#pragma unroll
-        for (int j = 0; j < 4; j++) x[i][j] = v[j], x[i][4 + j] = w[j];
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[i][j] = row < p.rows && col + j < p.cols ? (float)s[j] : 0.f;
-    }
-  }
+    for (int r = 0; r < 4; r++) load8<SRC>(p, br * 128 + rg * 4 + r + 64 * h, col, x[h][r]);
 
-  // the block's scale, for each element this thread holds
-  float inv[TILES ? 1 : TRANS ? 8 : kRows];
-  if constexpr (!TILES && !TRANS) {
-#pragma unroll
-    for (int i = 0; i < kRows; i++) {
-      unsigned m = 0;
-#pragma unroll
-      for (int j = 0; j < 8; j++) m = max(m, magnitude(x[i][j]));
-#pragma unroll
-      for (int off = 8; off; off >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, off, 16));
-      float scale;
-      scale_of(m, &scale, &inv[i]);
-      const int row = br * 128 + rg + 16 * i;
-      if (c16 == 0 && row < p.rows) p.scales[bc * p.ld_scales + row] = scale;
-    }
-  } else if constexpr (!TILES) {
+  float inv[TILES ? 1 : 8];
+  if constexpr (!TILES) {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       unsigned m = 0;
 #pragma unroll
-      for (int i = 0; i < kRows; i++) m = max(m, magnitude(x[i][j]));
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) m = max(m, magnitude(x[h][r][j]));
       red[rg][c16 * 8 + j] = m;
     }
     __syncthreads();
@@ -107,9 +151,9 @@ __global__ __launch_bounds__(256) void quantize_kernel(QuantArgs p) {
   } else {
     unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < kRows; i++)
+    for (int h = 0; h < 2; h++)
 #pragma unroll
-      for (int j = 0; j < 8; j++) m = max(m, magnitude(x[i][j]));
+      for (int r = 0; r < 4; r++) m = max(m, magnitude8(x[h][r]));
 #pragma unroll
     for (int off = 32; off; off >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, off, 64));
     if ((t & 63) == 0) red[0][t >> 6] = m;
@@ -120,47 +164,53 @@ __global__ __launch_bounds__(256) void quantize_kernel(QuantArgs p) {
     if (t == 0) p.scales[TRANS ? (int64_t)bc * p.ld_scales + br : (int64_t)br * p.ld_scales + bc] = scale;
   }
 
+  if constexpr (!TRANS) {
+    const int last16 = (p.cols + 15) & ~15;
 #pragma unroll
-  for (int i = 0; i < kRows; i++) {
-    unsigned w[2];
+    for (int h = 0; h < 2; h++)
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      float y[4];
+      for (int r = 0; r < 4; r++) {
+        const int row = br * 128 + rg * 4 + r + 64 * h;
+        const float(&v)[8] = x[h][r];
+        if (row < p.rows && col < last16)
+          *(u32x2*)(p.dst + (int64_t)row * p.ld_dst + col) = u32x2{e4m3x4(v[0] * inv[0], v[1] * inv[0], v[2] * inv[0], v[3] * inv[0]),
+                                                                   e4m3x4(v[4] * inv[0], v[5] * inv[0], v[6] * inv[0], v[7] * inv[0])};
+      }
+  } else {
 #pragma unroll
-      for (int j = 0; j < 4; j++) y[j] = x[i][4 * h + j] * inv[TILES ? 0 : TRANS ? 4 * h + j : i];
-      unsigned v = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-      w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], v, true);
-    }
-    if constexpr (!TRANS) {
-      // elements up to the next multiple of 16 columns are written, as zeros behind the last one
-      const int row = br * 128 + rg + 16 * i;
-      if (row < p.rows && col < ((p.cols + 15) & ~15)) *(u32x2*)(p.dst + (int64_t)row * p.ld_dst + col) = u32x2{w[0], w[1]};
-    } else {
+    for (int h = 0; h < 2; h++)
 #pragma unroll
-      for (int j = 0; j < 8; j++) turned[(c16 * 8 + j) * 144 + rg + 16 * i] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
-    }
-  }
-  if constexpr (TRANS) {
+      for (int j = 0; j < 8; j++) {
+        const float f = inv[TILES ? 0 : j];
+        const int chunk = (rg >> 2) + 4 * h;
+        turned[(c16 * 8 + j) * 32 + (chunk ^ (c16 & 7)) * 4 + (rg & 3)] = e4m3x4(x[h][0][j] * f, x[h][1][j] * f, x[h][2][j] * f, x[h][3][j] * f);
+      }
     __syncthreads();
     const int rows16 = (p.rows + 15) & ~15;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const int c = (t >> 3) + 32 * i, r = br * 128 + (t & 7) * 16;
+      const int c = (t >> 3) + 32 * i, chunk = t & 7, r = br * 128 + chunk * 16;
       if (bc * 128 + c < p.cols && r < rows16)
-        *(u32x4*)(p.dst + (int64_t)(bc * 128 + c) * p.ld_dst + r) = *(const u32x4*)(turned + c * 144 + (t & 7) * 16);
+        *(u32x4*)(p.dst + (int64_t)(bc * 128 + c) * p.ld_dst + r) = *(const u32x4*)(turned + c * 32 + (chunk ^ ((c >> 3) & 7)) * 4);
     }
   }
 }
 
 template <typename SRC>
-void launch_quantize(const QuantArgs& p, bool tiles, bool trans, unsigned grid, hipStream_t st) {
-  if (tiles) {
-    if (trans) quantize_kernel<SRC, true, true><<<grid, 256, 0, st>>>(p);
-    else quantize_kernel<SRC, true, false><<<grid, 256, 0, st>>>(p);
-  } else {
-    if (trans) quantize_kernel<SRC, false, true><<<grid, 256, 0, st>>>(p);
-    else quantize_kernel<SRC, false, false><<<grid, 256, 0, st>>>(p);
+int launch_quantize(const QuantArgs& p, bool tiles, bool trans, hipStream_t st) {
+  const bool rows = !tiles && !trans;
+  const int64_t grid = rows ? (int64_t)((p.rows + (int64_t)kRowsGroup - 1) / kRowsGroup) * ((p.cols + (int64_t)kColsGroup - 1) / kColsGroup)
+                            : ((p.rows + (int64_t)127) / 128) * ((p.cols + (int64_t)127) / 128);
+  if (grid > 0x7fffffff) {
+    gmd::set_error("block quantise: too many blocks for one launch");
+    return GMD_ERR_BADPARAM;
   }
+  if (rows) quantize_rows_kernel<SRC><<<(unsigned)grid, 256, 0, st>>>(p);
+  else if (!trans) quantize_region_kernel<SRC, true, false><<<(unsigned)grid, 256, 0, st>>>(p);
+  else if (tiles) quantize_region_kernel<SRC, true, true><<<(unsigned)grid, 256, 0, st>>>(p);
+  else quantize_region_kernel<SRC, false, true><<<(unsigned)grid, 256, 0, st>>>(p);
+  GMD_HIP(hipGetLastError());
+  return GMD_OK;
 }
 
 }  // namespace
@@ -190,12 +240,9 @@ int gmd_block_quantize_launch(const gmd_block_quantize_t* q, void* hip_stream) {
   if (p.ld_dst < c16 || p.ld_dst % 16) return refuse("a result row stride that is not a multiple of 16 or shorter than a row rounded up to 16");
   if (p.ld_scales < (q->blocks == GMD_BLOCK_ROWS ? r : kb)) return refuse("a stride of scales shorter than what it spans");
   p.vec = (((uintptr_t)p.src | (uintptr_t)(p.ld_src * elem)) & 15) == 0;
-  const int64_t grid = (((int64_t)q->rows + 127) / 128) * (((int64_t)q->cols + 127) / 128);
-  if (grid > 0x7fffffff) return refuse("too many blocks for one launch");
-  if (q->src_dtype == GMD_DT_BF16) launch_quantize<__bf16>(p, q->blocks == GMD_BLOCK_TILES, q->transpose != 0, (unsigned)grid, (hipStream_t)hip_stream);
-  else launch_quantize<float>(p, q->blocks == GMD_BLOCK_TILES, q->transpose != 0, (unsigned)grid, (hipStream_t)hip_stream);
-  GMD_HIP(hipGetLastError());
-  return GMD_OK;
+  const bool tiles = q->blocks == GMD_BLOCK_TILES, trans = q->transpose != 0;
+  return q->src_dtype == GMD_DT_BF16 ? launch_quantize<__bf16>(p, tiles, trans, (hipStream_t)hip_stream)
+                                     : launch_quantize<float>(p, tiles, trans, (hipStream_t)hip_stream);
 }
 
 }  // extern "C"
