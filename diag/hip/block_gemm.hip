@@ -5,43 +5,11 @@
 
 namespace gmd {
 namespace tiles {
-namespace {
-
-template <int KIND, int BM, int BN, int WM, int WN, typename OUT>
-int launch_tile(const Args& p, hipStream_t st) {
-  const int64_t grid = grid_of(p, BM, BN);
-  if (int rc = launched("block GEMM", grid)) return rc;
-  tile_kernel<KIND, false, false, false, BM, BN, WM, WN, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
-  GMD_HIP(hipGetLastError());
-  return GMD_OK;
-}
-
-template <int KIND, int MB, typename OUT>
-int launch_few(const Args& p, hipStream_t st) {
-  const int64_t grid = grid_of(p, MB * 16, 16);
-  if (int rc = launched("block GEMM", grid)) return rc;
-  few_rows_kernel<KIND, MB, OUT><<<(unsigned)grid, kFewWaves * 64, 0, st>>>(p);
-  GMD_HIP(hipGetLastError());
-  return GMD_OK;
-}
-
-template <int KIND, typename OUT>
-int launch_kind(const Args& p, hipStream_t st) {
-  // rows per product: all of them, or an expert's share on average (the host does not see the offsets)
-  const int rows = p.offsets ? (p.m + p.groups - 1) / p.groups : p.m;
-  if (rows <= 16) return launch_few<KIND, 1, OUT>(p, st);
-  if (rows <= 32) return launch_few<KIND, 2, OUT>(p, st);
-  if (rows <= 64) return launch_few<KIND, 4, OUT>(p, st);
-  if (sizeof(OUT) == 2 && grid_of(p, 256, 256) >= kCUs) return launch_tile<KIND, 256, 256, 2, 4, __bf16>(p, st);
-  return launch_tile<KIND, 128, 128, 2, 2, OUT>(p, st);
-}
-
-}  // namespace
 
 int launch_fp8(const Args& p, int b_blocks, int out_dtype, hipStream_t st) {
   if (b_blocks == GMD_BLOCK_TILES)
-    return out_dtype == GMD_DT_BF16 ? launch_kind<kFp8Tiles, __bf16>(p, st) : launch_kind<kFp8Tiles, float>(p, st);
-  return out_dtype == GMD_DT_BF16 ? launch_kind<kFp8Rows, __bf16>(p, st) : launch_kind<kFp8Rows, float>(p, st);
+    return out_dtype == GMD_DT_BF16 ? launch_forward<kFp8Tiles, __bf16>(p, st) : launch_forward<kFp8Tiles, float>(p, st);
+  return out_dtype == GMD_DT_BF16 ? launch_forward<kFp8Rows, __bf16>(p, st) : launch_forward<kFp8Rows, float>(p, st);
 }
 
 }  // namespace tiles

@@ -7,6 +7,7 @@
 // A K-step is 128 bytes of k: 64 bf16 or one block of 128 e4m3.
 #pragma once
 
+#include <cmath>
 #include <type_traits>
 
 #include "diag_common.h"
@@ -87,41 +88,39 @@ __device__ __forceinline__ bool find_tile(const Args& p, int bm, int bn, int id,
     return true;
   }
   const int lane = threadIdx.x & 63;
-  int total = 0;
-  for (int g0 = 0; g0 < p.groups; g0 += 64) {
-    int lo = 0, hi = 0;
+  int lo = 0, hi = 0, upto = 0;  // of expert g0 + lane; tiles up to and with it, among these 64
+  auto scan = [&](int g0) {
+    lo = hi = 0;
     if (g0 + lane < p.groups) group_rows(p.offsets, g0 + lane, p.m, &lo, &hi);
-    int tiles = (hi - lo + bm - 1) / bm;
-#pragma unroll
-    for (int off = 32; off; off >>= 1) tiles += __shfl_xor(tiles, off, 64);
-    total += tiles;
-  }
-  total = __builtin_amdgcn_readfirstlane(total);
-  if (id >= total * tiles_n) return false;
-  const int work = xcd_contiguous(id, total * tiles_n);
-  int before = 0;  // tiles of the experts in front
-  for (int g0 = 0; g0 < p.groups; g0 += 64) {
-    int lo = 0, hi = 0;
-    if (g0 + lane < p.groups) group_rows(p.offsets, g0 + lane, p.m, &lo, &hi);
-    const int mine = (hi - lo + bm - 1) / bm * tiles_n;
-    int upto = mine;
+    upto = (hi - lo + bm - 1) / bm * tiles_n;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const int v = __shfl_up(upto, off, 64);
       if (lane >= off) upto += v;
     }
+  };
+  int total = 0;
+  for (int g0 = 0; g0 < p.groups; g0 += 64) {
+    scan(g0);
+    total += __builtin_amdgcn_readlane(upto, 63);
+  }
+  if (id >= total) return false;
+  const int work = xcd_contiguous(id, total);
+  int before = 0;  // tiles of the experts in front
+  for (int g0 = 0; g0 < p.groups; g0 += 64) {
+    if (p.groups > 64) scan(g0);  // up to 64 are still there
     const int in = work - before;
     const unsigned long long has = __ballot(in < upto);
     if (has) {
       const int l = __builtin_ctzll(has);  // the first expert whose tiles reach past this one
-      const int glo = __builtin_amdgcn_readfirstlane(__shfl(lo, l, 64)), ghi = __builtin_amdgcn_readfirstlane(__shfl(hi, l, 64));
-      const int first = __builtin_amdgcn_readfirstlane(__shfl(upto - mine, l, 64));
+      const int glo = __builtin_amdgcn_readlane(lo, l), ghi = __builtin_amdgcn_readlane(hi, l);
+      const int tiles_m = (ghi - glo + bm - 1) / bm, first = __builtin_amdgcn_readlane(upto, l) - tiles_m * tiles_n;
       int tm, tn;
-      tile_walk(in - first, (ghi - glo + bm - 1) / bm, tiles_n, &tm, &tn);
+      tile_walk(in - first, tiles_m, tiles_n, &tm, &tn);
       t->group = g0 + l, t->m0 = glo + tm * bm, t->m_end = ghi, t->n0 = tn * bn;
       return true;
     }
-    before += __builtin_amdgcn_readfirstlane(__shfl(upto, 63, 64));
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
   return false;
 }
@@ -139,6 +138,7 @@ __device__ __forceinline__ int chunk_swizzle(int row) { return ((row >> 1) & 3) 
 // unit ^ unit_swizzle(row) so that these eight units lie in different banks (64 banks of 4 bytes).  COLS: columns of the image.
 template <int COLS>
 __device__ __forceinline__ int unit_swizzle(int row) {
+  static_assert(COLS >= 32, "two units at least");
   if constexpr (COLS >= 128) return ((row >> 3) & 1) * 4 + (row & 3);
   if constexpr (COLS == 64) return ((row >> 3) & 1) * 2 + ((row >> 1) & 1);
   return (row >> 3) & 1;
@@ -309,20 +309,20 @@ struct Operand<2> {
   }
 };
 
-// Eight f32 of a row -> C: one 16-byte store of bf16 or two of f32.  C is not read again by this kernel.
+// 16 bytes of a row of C, eight bf16 or four f32.  (Stored past the caches: no difference, 32k x 4096 x 2048 bf16 over 32 experts.)
 template <typename OUT>
-__device__ __forceinline__ void store8(OUT* dst, const f32x4& x, const f32x4& y) {
+__device__ __forceinline__ void store16(OUT* dst, const char* f32s) {
+  u32x4 o;
   if constexpr (sizeof(OUT) == 2) {
-    u32x4 o;
+    const f32x4 x = *(const f32x4*)f32s, y = *(const f32x4*)(f32s + 16);
     o[0] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{x[0], x[1]}, bf16x2));
     o[1] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{x[2], x[3]}, bf16x2));
     o[2] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{y[0], y[1]}, bf16x2));
     o[3] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{y[2], y[3]}, bf16x2));
-    *(u32x4*)dst = o;
   } else {
-    *(f32x4*)dst = x;
-    *(f32x4*)(dst + 4) = y;
+    o = *(const u32x4*)f32s;
   }
+  *(u32x4*)dst = o;
 }
 
 // ------------------------------------------------------------------------------------------------------ tile kernel --
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   static_assert(kWaves * 16 * kStrip <= 2 * kBufBytes, "the epilogue's strips fit into the operand buffers");
   constexpr int kScaleBytes = kFp8 ? kWaves * 256 : 0;
   static_assert(BM / 64 + (KIND == kFp8Rows ? BN / 64 : 1) <= kWaves, "one DMA of scales per wave and step");
-  __shared__ __attribute__((aligned(16))) char smem[2 * kBufBytes + 2 * kScaleBytes];
+  __shared__ __attribute__((aligned(16))) char smem[2 * (kBufBytes + kScaleBytes)];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -353,11 +353,14 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   int64_t k_first = 0;
   int K = p.k;
   if constexpr (WGRAD) {
-    const int tiles_m = (p.m + BM - 1) / BM, tiles_n = (p.n + BN - 1) / BN;
-    const int work = xcd_contiguous(blockIdx.x, gridDim.x);
+    // Every XCD takes an eighth of every expert's tiles, neighbours of the walk: the experts' numbers of rows differ, and with
+    // them what a tile costs (whole experts dealt to XCDs: GMD_WGRAD_BY_EXPERT us against GMD_WGRAD_EIGHTHS, 16k rows over 16 experts of 4096 x 2048).
+    const int tiles_m = (p.m + BM - 1) / BM, tiles_n = (p.n + BN - 1) / BN, eighth = (tiles_m * tiles_n + 7) / 8;
+    const int slot = (int)blockIdx.x >> 3, work = ((int)blockIdx.x & 7) * eighth + slot % eighth;
+    if (work >= tiles_m * tiles_n) return;
     int tm, tn, lo, hi;
-    t.group = work / (tiles_m * tiles_n);
-    tile_walk(work - t.group * tiles_m * tiles_n, tiles_m, tiles_n, &tm, &tn);
+    t.group = slot / eighth;
+    tile_walk(work, tiles_m, tiles_n, &tm, &tn);
     t.m0 = tm * BM, t.m_end = p.m, t.n0 = tn * BN;
     group_rows(p.offsets, t.group, p.k, &lo, &hi);
     k_first = lo, K = hi - lo;
@@ -412,10 +415,9 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   auto read_scales = [&](int kt) {
     const float* const q = (const float*)(smem + 2 * kBufBytes + (kt & 1) * kScaleBytes);
 #pragma unroll
-    for (int i = 0; i < MB; i += 4) {
-      const f32x4 v = *(const f32x4*)(q + wm * WTM + fr * MB + i);
-#pragma unroll
-      for (int r = 0; r < 4; r++) sl[i + r] = v[r];
+    for (int i = 0; i < MB; i += 2) {
+      const f32x2 v = *(const f32x2*)(q + wm * WTM + fr * MB + i);
+      sl[i] = v[0], sl[i + 1] = v[1];
     }
     if constexpr (KIND == kFp8Tiles) {
       sb[0][0] = q[BM + wn * WTN / 128];
@@ -467,7 +469,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   // 8192^3 block-scaled 505 us.
   constexpr int kProducts = MB * NB, kTail = (MB - 2) * NB, kHalf = NB / 2, kBar = kTail + kHalf, kMid = (MB / 2 - 1) * NB;
   constexpr int kPer = (kFirst + kBar - kMid - 1) / (kBar - kMid);  // DMAs behind one product, all of the first group before kBar
-  static_assert(MB >= 4 && MB % 2 == 0 && NB == 4 && kSecond <= kProducts - kBar, "the pieces fit behind the products");
+  static_assert(MB % 2 == 0 && NB == 4 && kSecond <= kProducts - kBar, "the pieces fit behind the products");
   auto row_of = [](int at) { return at < kTail ? at / NB : MB - 2 + (at - kTail) / kHalf % 2; };
   auto col_of = [](int at) { return at < kTail ? at % NB : (at - kTail) % kHalf + (at - kTail >= NB ? kHalf : 0); };
   typedef Operand<kFp8 ? (kNarrow ? 1 : 2) : 0> Op;
@@ -492,14 +494,13 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   };
   const std::integral_constant<int, 0> none;
   const std::integral_constant<int, kFirst + kSecond> step_behind;
-  const std::integral_constant<int, kSecond> second_behind;
   if (steps > 0) {
     fetch_edge(0, 0, kFirst + kSecond);
     if (steps > 1) {
       fetch_edge(1, 0, kFirst + kSecond);
       sync(std::integral_constant<int, kFirst + 2 * kSecond>());
     } else {
-      sync(second_behind);
+      sync(none);
     }
 #pragma unroll
     for (int j = 0; j < NB; j++) {
@@ -520,7 +521,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
     const char* const la = smem + (kt & 1) * kBufBytes;
     const char* const na = smem + ((kt + 1) & 1) * kBufBytes;
     const char* const nb = na + kABytes;
-    const bool more = kFull || kt + 1 < steps, more2 = kFull || kt + 2 < steps;
+    const bool more = kFull || kt + 1 < steps, more2 = kFull || kt + 2 < steps;  // (in flight behind kMid's and kBar's)
     const char* const src_a = ga.step_base(kt + 2);
     const char* const src_b = gb.step_base(kt + 2);
 #pragma unroll
@@ -584,7 +585,8 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   // neighbouring columns of one row.
   char* const strip = smem + wave * 16 * kStrip;
   OUT* const C = (OUT*)p.c + (WGRAD ? t.group * p.stride_c : 0);
-  constexpr int kLanesPerRow = WTN / 8, kRowsPerPass = 64 / kLanesPerRow;
+  constexpr int kCols16 = 16 / (int)sizeof(OUT);  // columns of a 16-byte store
+  constexpr int kLanesPerRow = WTN / kCols16, kRowsPerPass = 64 / kLanesPerRow;
 #pragma unroll
   for (int i = 0; i < MB; i++) {
 #pragma unroll
@@ -593,10 +595,9 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int r0 = 0; r0 < 16; r0 += kRowsPerPass) {
-      const int f = r0 + lane / kLanesPerRow, c8 = lane % kLanesPerRow * 8;
-      const f32x4 x = *(const f32x4*)(strip + f * kStrip + c8 * 4), y = *(const f32x4*)(strip + f * kStrip + c8 * 4 + 16);
-      const int row = t.m0 + wm * WTM + (kFp8 ? f * MB + i : i * 16 + f), col = t.n0 + wn * WTN + c8;
-      if (row < t.m_end && col < p.n) store8<OUT>(C + row * p.ldc + col, x, y);  // N is a multiple of 8
+      const int f = r0 + lane / kLanesPerRow, c = lane % kLanesPerRow * kCols16;
+      const int row = t.m0 + wm * WTM + (kFp8 ? f * MB + i : i * 16 + f), col = t.n0 + wn * WTN + c;
+      if (row < t.m_end && col < p.n) store16<OUT>(C + row * p.ldc + col, strip + f * kStrip + c * 4);  // N is a multiple of 8
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -604,94 +605,129 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
 }
 
 // ---------------------------------------------------------------------------------------------------- few-row kernel --
-// Up to 16 MB rows x 16 columns per workgroup: what bounds such a product is reading B once, so B goes straight from memory
-// to the registers that the MFMA takes (lane (fr, fq): row fr, chunks fq and 4 + fq of the 128 bytes) and the eight waves
-// share the K-steps in turn, four at a time in flight each.  Their sums are joined in LDS in the order of the waves.
-constexpr int kFewWaves = 8;
-template <int KIND, int MB, typename OUT>
-__global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(Args p) {
+// 16 MB rows by 16 NB columns per workgroup, whose W waves share the K-steps in turn.  What bounds a product of few rows is the
+// rate at which operands come in, and the tile above leaves most of the chip idle: here K is spread over the waves, every wave
+// walks its own steps through a ring of U slots of LDS that no other wave touches (no barrier until the end), and the W sums
+// are joined in LDS in the order of the waves.
+// Through LDS and not straight into registers because of the address path: it takes a quad of lanes that asks for 64
+// contiguous bytes in one cycle, but lanes of an MFMA operand are neighbours in different rows, one lane a cycle (64 rows of
+// 512 x 8192 e4m3: GMD_US_DIRECT us loaded directly, GMD_US_LDS this way).
+template <int KIND, int MB, int NB, int W, int U, typename OUT>
+__global__ __launch_bounds__(W * 64) void few_rows_kernel(Args p) {
   constexpr bool kFp8 = KIND != kBf16, kNarrow = sizeof(OUT) == 2;
   constexpr int kElem = kFp8 ? 1 : 2;
-  constexpr int U = MB <= 2 ? 4 : 2;
-  __shared__ f32x4 sums[kFewWaves][MB][64];
+  constexpr int kPieces = 2 * (MB + NB), kScaleDmas = !kFp8 ? 0 : KIND == kFp8Rows ? 2 : 1, kDmas = kPieces + kScaleDmas;
+  constexpr int kSlot = kPieces * 1024 + kScaleDmas * 256;
+  static_assert(MB <= 4 && NB <= 4 && 128 % (NB * 16) == 0, "a step's scales in one DMA each, the columns inside one tile of scales");
+  static_assert((U - 1) * kDmas < 64 && W * MB * NB * 1024 <= W * U * kSlot, "vmcnt counts to 63; the sums fit into the ring");
+  __shared__ __attribute__((aligned(16))) char smem[W * U * kSlot];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Tile t;
-  if (!find_tile(p, MB * 16, 16, blockIdx.x, &t)) return;
+  if (!find_tile(p, MB * 16, NB * 16, blockIdx.x, &t)) return;
   const int kbytes = p.k * kElem;
   const int steps = (kbytes + kStepBytes - 1) / kStepBytes;
-  const char* const zero = (const char*)&g_zero16;
-  const char* const b_row = p.b + t.group * p.stride_b + (int64_t)min(t.n0 + fr, p.n - 1) * p.ldb + fq * 16;
-  const char* a_row[MB];
-  int row[MB];
-#pragma unroll
-  for (int i = 0; i < MB; i++) {
-    row[i] = min(t.m0 + i * 16 + fr, t.m_end - 1);
-    a_row[i] = p.a + (int64_t)row[i] * p.lda + fq * 16;
-  }
-  const float* const SB = kFp8 ? p.sb + t.group * p.stride_sb : nullptr;
-  const int col4 = min(t.n0 + fq * 4, p.n - 4);
-  f32x4 acc[MB];
-#pragma unroll
-  for (int i = 0; i < MB; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int mine = steps > wave ? (steps - wave + W - 1) / W : 0;  // this wave's: wave, wave + W, ...
+  char* const ring = smem + wave * U * kSlot;
 
-  auto load2 = [&](const char* q, int kt, i32x4* lo, i32x4* hi) {
-    const int at = kt * kStepBytes + fq * 16;  // byte of k of the first chunk; the second is 64 further on
-    const char* r = q + (int64_t)kt * kStepBytes;
-    *lo = *(const i32x4*)(at < kbytes ? r : zero);
-    *hi = *(const i32x4*)(at + 64 < kbytes ? r + 64 : zero);
-  };
-  for (int k0 = wave; k0 < steps; k0 += kFewWaves * U) {
-    i32x4 bl[U], bh[U], al[U][MB], ah[U][MB];
-    float sa[U][MB];
-    f32x4 sb[U];
+  // Piece i: rows 8 i .. 8 i + 7 of A and then of B, 128 bytes each; rows beyond the last repeat it.
+  const char* const a_base = p.a + (int64_t)t.m0 * p.lda;
+  const char* const b_base = p.b + t.group * p.stride_b + (int64_t)t.n0 * p.ldb;
+  uint32_t off[kPieces];
+  const int chunk = (lane & 7) ^ chunk_swizzle(lane >> 3);
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int kt = k0 + u * kFewWaves;
-      if (kt < steps) {
-        load2(b_row, kt, &bl[u], &bh[u]);
-#pragma unroll
-        for (int i = 0; i < MB; i++) load2(a_row[i], kt, &al[u][i], &ah[u][i]);
-        if constexpr (kFp8) {
-#pragma unroll
-          for (int i = 0; i < MB; i++) sa[u][i] = p.sa[kt * p.ld_sa + row[i]];
-          if constexpr (KIND == kFp8Tiles) {
-            sb[u][0] = SB[(int64_t)(t.n0 / 128) * p.ld_sb + kt];
-          } else {
-            const float* r = SB + kt * p.ld_sb + col4;
-            sb[u] = f32x4{r[0], r[1], r[2], r[3]};
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (k0 + u * kFewWaves >= steps) break;
-      Operand<kNarrow ? 1 : 2> bf;
-      if constexpr (kFp8) bf.set(bl[u], bh[u]);
-#pragma unroll
-      for (int i = 0; i < MB; i++) {
-        if constexpr (kFp8) {
-          Operand<kNarrow ? 1 : 2> af;
-          af.set(al[u][i], ah[u][i]);
-          const f32x4 part = Operand<kNarrow ? 1 : 2>::product(bf, af);
-#pragma unroll
-          for (int r = 0; r < 4; r++) acc[i][r] = __builtin_fmaf(sa[u][i] * (KIND == kFp8Tiles ? sb[u][0] : sb[u][r]), part[r], acc[i][r]);
-        } else {
-          acc[i] = mfma_bf16(bl[u], al[u][i], acc[i]);
-          acc[i] = mfma_bf16(bh[u], ah[u][i], acc[i]);
-        }
-      }
-    }
+  for (int i = 0; i < kPieces; i++) {
+    const int r = i * 8 + (lane >> 3);
+    off[i] = (uint32_t)(r < MB * 16 ? min(r, t.m_end - 1 - t.m0) * p.lda : min(r - MB * 16, p.n - 1 - t.n0) * p.ldb) + chunk * 16;
   }
+  const float* const sa_base = kFp8 ? p.sa + t.m0 : nullptr;
+  const uint32_t sa_off = (uint32_t)min(lane, t.m_end - 1 - t.m0) * 4;
+  const float* const SB = !kFp8 ? nullptr : p.sb + t.group * p.stride_sb + (KIND == kFp8Rows ? (int64_t)t.n0 : (int64_t)(t.n0 / 128) * p.ld_sb);
+  const uint32_t sb_off = (uint32_t)min(lane, p.n - 1 - t.n0) * 4;
+  auto issue = [&](int s) {
+    const int kt = wave + s * W;
+    char* const slot = ring + s % U * kSlot;
+    const char* const at_a = a_base + (int64_t)kt * kStepBytes;
+    const char* const at_b = b_base + (int64_t)kt * kStepBytes;
+    if ((kt + 1) * kStepBytes <= kbytes) {
 #pragma unroll
-  for (int i = 0; i < MB; i++) sums[wave][i][lane] = acc[i];
+      for (int i = 0; i < kPieces; i++) dma<16>(i < 2 * MB ? at_a : at_b, off[i], slot + i * 1024);
+    } else {  // K ends inside this step: zeros behind it
+      const bool in = kt * kStepBytes + chunk * 16 < kbytes;
+#pragma unroll
+      for (int i = 0; i < kPieces; i++)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(in ? (i < 2 * MB ? at_a : at_b) + off[i] : (const char*)&g_zero16),
+                                         (__attribute__((address_space(3))) void*)(slot + i * 1024), 16, 0, 0);
+    }
+    if constexpr (kFp8) dma<4>(sa_base + kt * p.ld_sa, sa_off, slot + kPieces * 1024);
+    if constexpr (KIND == kFp8Rows) dma<4>(SB + kt * p.ld_sb, sb_off, slot + kPieces * 1024 + 256);
+  };
+  f32x4 acc[MB][NB];
+#pragma unroll
+  for (int i = 0; i < MB; i++)
+#pragma unroll
+    for (int j = 0; j < NB; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Frags<false, 16, 1, 0> frag;
+  frag.init(0, lane);
+
+#pragma unroll
+  for (int u = 0; u < U; u++)
+    if (u < mine) issue(u);
+  for (int s = 0; s < mine; s++) {
+    // the oldest slot has landed: the U - 1 behind it may be in flight
+    if (s + U <= mine) __builtin_amdgcn_s_waitcnt(((U - 1) * kDmas & 15) | 0xf70 | ((U - 1) * kDmas >> 4) << 14);
+    else __builtin_amdgcn_s_waitcnt(0xf70);
+    asm volatile("" ::: "memory");
+    const char* const slot = ring + s % U * kSlot;
+    Operand<kFp8 ? (kNarrow ? 1 : 2) : 0> af[MB], bf[NB];
+#pragma unroll
+    for (int j = 0; j < NB; j++) bf[j].set(frag.read(slot, MB + j, 0), frag.read(slot, MB + j, 1));
+#pragma unroll
+    for (int i = 0; i < MB; i++) af[i].set(frag.read(slot, i, 0), frag.read(slot, i, 1));
+    float sa[MB];
+    f32x4 sb[KIND == kFp8Rows ? NB : 1];
+    if constexpr (kFp8) {
+      const float* const q = (const float*)(slot + kPieces * 1024);
+#pragma unroll
+      for (int i = 0; i < MB; i++) sa[i] = q[i * 16 + fr];
+      if constexpr (KIND == kFp8Tiles) {
+        sb[0][0] = ((const __attribute__((address_space(4))) float*)SB)[wave + s * W];  // one scalar load
+      } else {
+#pragma unroll
+        for (int j = 0; j < NB; j++) sb[j] = *(const f32x4*)(q + 64 + j * 16 + fq * 4);
+      }
+    }
+    if (s + U < mine) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the slot has been read and can be refilled
+      asm volatile("" ::: "memory");
+      issue(s + U);
+    }
+#pragma unroll
+    for (int i = 0; i < MB; i++)
+#pragma unroll
+      for (int j = 0; j < NB; j++) {
+        if constexpr (kFp8) {
+          const f32x4 part = Operand<kNarrow ? 1 : 2>::product(bf[j], af[i]);
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            acc[i][j][r] = __builtin_fmaf(sa[i] * (KIND == kFp8Tiles ? sb[0][0] : sb[KIND == kFp8Tiles ? 0 : j][r]), part[r], acc[i][j][r]);
+        } else {
+          Operand<0>::accumulate(bf[j], af[i], acc[i][j]);
+        }
+      }
+  }
   __syncthreads();
-  if (wave < MB) {  // wave i joins block i: lane (fr, fq) holds row fr, columns 4 fq ..
-    f32x4 v = sums[0][wave][lane];
+  f32x4* const sums = (f32x4*)smem;  // [wave][block][lane]
 #pragma unroll
-    for (int w = 1; w < kFewWaves; w++) v += sums[w][wave][lane];
-    const int r = t.m0 + wave * 16 + fr, col = t.n0 + fq * 4;
+  for (int i = 0; i < MB; i++)
+#pragma unroll
+    for (int j = 0; j < NB; j++) sums[(wave * MB * NB + i * NB + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  for (int q = wave; q < MB * NB; q += W) {
+    f32x4 v = sums[q * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < W; w++) v += sums[(w * MB * NB + q) * 64 + lane];
+    const int r = t.m0 + q / NB * 16 + fr, col = t.n0 + q % NB * 16 + fq * 4;
     if (r < t.m_end && col < p.n) {
       OUT* dst = (OUT*)p.c + r * p.ldc + col;
       if constexpr (sizeof(OUT) == 2) *(bf16x4*)dst = __builtin_convertvector(v, bf16x4);
@@ -713,6 +749,80 @@ inline int launched(const char* what, int64_t grid) {
     return GMD_ERR_BADPARAM;
   }
   return GMD_OK;
+}
+
+// The K-contiguous product (forward, and every block-scaled one): which kernel.
+// `rows` is what one product has: all of them, or an expert's share on average (the host does not see the offsets).
+// * The few-row kernel gives a workgroup 16 MB x 16 NB of C with K spread over its waves.  MB covers the rows (one block of 16, two
+//   or four); NB is the smallest of 1, 2 and 4 whose grid still fits the chip at one workgroup a CU: every doubling of NB halves
+//   the times A is read, but a CU without a workgroup is lost (32 x 4096 x 7168 e4m3: NB 1 9.9 us, NB 2 12.0; 32 x 7168 x 2048: 8.2 and 6.0).
+//   Past that, NB 4, up to 32 rows always, since what is read then is B, once; with more rows tiles are faster (128 x 7168 x 2048:
+//   9.8 against 14.6 us, 200 x 7168 x 2048: 16.7 against 14.2).
+// * Experts with up to 32 rows on average take it as well, in workgroups of four waves so that several fit on a CU and hide each
+//   other's start: 64 experts of 2048 x 2048 bf16 for 64 rows 43.4 us (tiles 58.5), for 2048 rows 62 (65.6).
+// * Tiles of 128 x 128 with eight waves, two workgroups a CU, or of 256 x 256, one a CU: by a model of their rounds over the chip, fitted
+//   on 2048 x 4096 x 4096 (42 against 54 us), 2048 x 7168 x 512 (18 against 15) and 8192^3 (646 against 430).
+struct TileCost {
+  static double small(double tiles, double steps) {  // rounds of 512; half a round or less runs alone on its CUs
+    const double full = std::floor(tiles / 512), rest = tiles - 512 * full;
+    return full * (1.2 * steps + 4) + (rest > 256 ? 1.2 * steps + 4 : rest > 0 ? 0.6 * steps + 4 : 0);
+  }
+  static double large(double tiles, double steps) { return std::ceil(tiles / 256) * (1.55 * steps + 8); }
+};
+// Tiles that a launch really has: with experts about half a row of tiles each is cut off.
+inline double tiles_of(const Args& p, int bm, int bn) {
+  const double rows = p.offsets ? p.m / (double)bm + 0.5 * std::min(p.groups, p.m) : std::ceil(p.m / (double)bm);
+  return rows * std::ceil(p.n / (double)bn);
+}
+inline bool large_tiles(const Args& p, int step_k) {
+  const double steps = std::ceil(p.k / (double)step_k);
+  return TileCost::large(tiles_of(p, 256, 256), steps) < TileCost::small(tiles_of(p, 128, 128), steps);
+}
+
+template <int KIND, bool TA, bool TB, int BM, int BN, int WM, int WN, typename OUT>
+int launch_tile(const Args& p, hipStream_t st) {
+  constexpr bool kWgrad = TA;
+  const int64_t tiles = (((int64_t)p.m + BM - 1) / BM) * (((int64_t)p.n + BN - 1) / BN);
+  const int64_t grid = kWgrad ? p.groups * ((tiles + 7) / 8 * 8) : grid_of(p, BM, BN);
+  if (int rc = launched("GEMM", grid)) return rc;
+  tile_kernel<KIND, TA, TB, kWgrad, BM, BN, WM, WN, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
+  GMD_HIP(hipGetLastError());
+  return GMD_OK;
+}
+template <int KIND, int MB, int NB, int W, int U, typename OUT>
+int launch_few(const Args& p, hipStream_t st) {
+  const int64_t grid = grid_of(p, MB * 16, NB * 16);
+  if (int rc = launched("GEMM", grid)) return rc;
+  few_rows_kernel<KIND, MB, NB, W, U, OUT><<<(unsigned)grid, W * 64, 0, st>>>(p);
+  GMD_HIP(hipGetLastError());
+  return GMD_OK;
+}
+template <int KIND, typename OUT>
+int launch_forward(const Args& p, hipStream_t st) {
+  const int rows = p.offsets ? (p.m + p.groups - 1) / p.groups : p.m;
+  const int mb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int nb = grid_of(p, 16 * mb, 16) <= kCUs ? 1 : grid_of(p, 16 * mb, 32) <= kCUs ? 2 : grid_of(p, 16 * mb, 64) <= kCUs ? 4 : 0;
+  if (mb == 1) {
+    if (nb == 1) return launch_few<KIND, 1, 1, 8, 2, OUT>(p, st);
+    // (e4m3 experts: a slot less in flight leaves room for twice the workgroups, 128 experts of 2048 x 1024 for 128 rows 42 -> 34 us)
+    if (p.offsets) return KIND == kBf16 ? launch_few<KIND, 1, 2, 4, 2, OUT>(p, st) : launch_few<KIND, 1, 2, 4, 1, OUT>(p, st);
+    return nb == 2 ? launch_few<KIND, 1, 2, 4, 2, OUT>(p, st) : launch_few<KIND, 1, 4, 4, 2, OUT>(p, st);
+  }
+  if (mb == 2) {
+    if (nb == 1) return launch_few<KIND, 2, 1, 8, 2, OUT>(p, st);
+    if (p.offsets) return launch_few<KIND, 2, 4, 4, 1, OUT>(p, st);
+    return nb == 2 ? launch_few<KIND, 2, 2, 4, 2, OUT>(p, st) : launch_few<KIND, 2, 4, 4, 2, OUT>(p, st);
+  }
+  if (nb == 1) return launch_few<KIND, 4, 1, 6, 2, OUT>(p, st);
+  if (nb == 2) return launch_few<KIND, 4, 2, 8, 1, OUT>(p, st);
+  if (nb == 4) return launch_few<KIND, 4, 4, 4, 2, OUT>(p, st);
+  // (f32 results of e4m3 operands are computed on widened fragments, which do not fit the large tile's registers)
+  if constexpr (KIND == kBf16 || sizeof(OUT) == 2)
+    if (large_tiles(p, KIND == kBf16 ? 64 : 128)) return launch_tile<KIND, false, false, 256, 256, 2, 4, OUT>(p, st);
+  // (widening costs a wave per fragment, not per product: four waves of 64 x 64 have fewer of them per product than eight of 32 x 64,
+  // 2048 x 7168 x 8192 276 against 326 us)
+  if constexpr (KIND != kBf16 && sizeof(OUT) == 4) return launch_tile<KIND, false, false, 128, 128, 2, 2, OUT>(p, st);
+  else return launch_tile<KIND, false, false, 128, 128, 4, 2, OUT>(p, st);
 }
 
 // Block-scaled fp8, one product or one per expert (block_gemm.hip).

@@ -9,40 +9,17 @@ namespace gmd {
 namespace tiles {
 namespace {
 
-template <bool TA, bool TB, bool WGRAD, int BM, int BN, int WM, int WN, typename OUT>
-int launch_tile(const Args& p, hipStream_t st) {
-  const int64_t grid = WGRAD ? (int64_t)p.groups * ((p.m + BM - 1) / BM) * ((p.n + BN - 1) / BN) : grid_of(p, BM, BN);
-  if (int rc = launched("grouped GEMM", grid)) return rc;
-  tile_kernel<kBf16, TA, TB, WGRAD, BM, BN, WM, WN, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
-  GMD_HIP(hipGetLastError());
-  return GMD_OK;
-}
-
-template <int MB, typename OUT>
-int launch_few(const Args& p, hipStream_t st) {
-  const int64_t grid = grid_of(p, MB * 16, 16);
-  if (int rc = launched("grouped GEMM", grid)) return rc;
-  few_rows_kernel<kBf16, MB, OUT><<<(unsigned)grid, kFewWaves * 64, 0, st>>>(p);
-  GMD_HIP(hipGetLastError());
-  return GMD_OK;
-}
-
 template <typename OUT>
 int launch_bf16(int op, const Args& p, hipStream_t st) {
-  const int rows = (p.m + p.groups - 1) / p.groups;  // an expert's share on average
-  if (op == GMD_GROUPED_FORWARD) {
-    if (rows <= 16) return launch_few<1, OUT>(p, st);
-    if (rows <= 32) return launch_few<2, OUT>(p, st);
-    if (rows <= 64) return launch_few<4, OUT>(p, st);
-    if (grid_of(p, 256, 256) >= kCUs) return launch_tile<false, false, false, 256, 256, 2, 4, OUT>(p, st);
-    return launch_tile<false, false, false, 128, 128, 2, 2, OUT>(p, st);
-  }
-  if (op == GMD_GROUPED_DGRAD) {
-    if (rows > 64 && grid_of(p, 256, 256) >= kCUs) return launch_tile<false, true, false, 256, 256, 2, 4, OUT>(p, st);
-    return launch_tile<false, true, false, 128, 128, 2, 2, OUT>(p, st);
-  }
-  if ((int64_t)p.groups * (p.m / 256) * (p.n / 256) >= kCUs) return launch_tile<true, true, true, 256, 256, 2, 4, OUT>(p, st);
-  return launch_tile<true, true, true, 128, 128, 2, 2, OUT>(p, st);
+  if (op == GMD_GROUPED_FORWARD) return launch_forward<kBf16, OUT>(p, st);
+  if (op == GMD_GROUPED_DGRAD)
+    return large_tiles(p, 64) ? launch_tile<kBf16, false, true, 256, 256, 2, 4, OUT>(p, st) : launch_tile<kBf16, false, true, 128, 128, 4, 2, OUT>(p, st);
+  Args one = p;  // an expert's share of the rows is its contraction
+  one.offsets = nullptr, one.k = (p.k + p.groups - 1) / p.groups, one.m = p.m;
+  const double steps = std::ceil(one.k / 64.0);
+  return TileCost::large(p.groups * tiles_of(one, 256, 256), steps) < TileCost::small(p.groups * tiles_of(one, 128, 128), steps)
+             ? launch_tile<kBf16, true, true, 256, 256, 2, 4, OUT>(p, st)
+             : launch_tile<kBf16, true, true, 128, 128, 2, 2, OUT>(p, st);
 }
 
 }  // namespace

@@ -5,6 +5,7 @@ every function here runs the HIP kernels of diag/hip (never a torch stand-in).
 torch is only ever used by callers as an *oracle* to check numerics.
 """
 import ctypes as C
+import struct
 
 from .._lib import diag_lib
 
@@ -91,9 +92,9 @@ def _lib():
         L.gmd_gemm_launch_mx.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                          C.c_void_p]
         L.gmd_mx_pack_scales.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]
-        L.gmd_block_quantize_launch.argtypes = [C.POINTER(BlockQuantize), C.c_void_p]
-        L.gmd_gemm_block_launch.argtypes = [C.POINTER(GemmBlock), C.c_void_p]
-        L.gmd_grouped_gemm_launch.argtypes = [C.POINTER(GroupedGemm), C.c_void_p]
+        L.gmd_block_quantize_launch.argtypes = [C.c_char_p, C.c_void_p]
+        L.gmd_gemm_block_launch.argtypes = [C.c_char_p, C.c_void_p]
+        L.gmd_grouped_gemm_launch.argtypes = [C.c_char_p, C.c_void_p]
         _typed = True
     return L
 
@@ -540,25 +541,21 @@ BLOCKS = {"rows": 0, "tiles": 1}
 GROUPED_OPS = {"forward": 0, "dgrad": 1, "wgrad": 2}
 
 
-class BlockQuantize(C.Structure):
-    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("scales", C.c_void_p), ("ld_src", C.c_int64),
-                ("ld_dst", C.c_int64), ("ld_scales", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32),
-                ("src_dtype", C.c_int32), ("blocks", C.c_int32), ("transpose", C.c_int32), ("reserved", C.c_int32)]
+# The three structs below are packed by hand, in the order of gpumon_diag.h: a ctypes.Structure per call costs as much host time as the
+# launch itself (2.6 against 0.6 us).
+_BLOCK_QUANTIZE = struct.Struct("3P3q6i")  # gmd_block_quantize_t
+_GEMM_BLOCK = struct.Struct("5P5q6i")      # gmd_gemm_block_t
+_GROUPED_GEMM = struct.Struct("6P7q8i")    # gmd_grouped_gemm_t
 
 
-class GemmBlock(C.Structure):
-    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("c", C.c_void_p), ("scale_a", C.c_void_p),
-                ("scale_b", C.c_void_p), ("lda", C.c_int64), ("ldb", C.c_int64), ("ldc", C.c_int64),
-                ("ld_scale_a", C.c_int64), ("ld_scale_b", C.c_int64), ("m", C.c_int32), ("n", C.c_int32),
-                ("k", C.c_int32), ("b_blocks", C.c_int32), ("out_dtype", C.c_int32), ("reserved", C.c_int32)]
-
-
-class GroupedGemm(C.Structure):
-    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("c", C.c_void_p), ("offsets", C.c_void_p),
-                ("scale_a", C.c_void_p), ("scale_b", C.c_void_p), ("lda", C.c_int64), ("ldb", C.c_int64),
-                ("ldc", C.c_int64), ("stride_w", C.c_int64), ("ld_scale_a", C.c_int64), ("ld_scale_b", C.c_int64),
-                ("stride_scale", C.c_int64), ("op", C.c_int32), ("dtype", C.c_int32), ("out_dtype", C.c_int32),
-                ("groups", C.c_int32), ("rows", C.c_int32), ("n", C.c_int32), ("k", C.c_int32), ("reserved", C.c_int32)]
+def _packed_launch(name, form, stream, *fields):
+    try:
+        packed = form.pack(*fields)
+    except struct.error as e:  # a size that its field cannot hold
+        raise DiagError(-1, f"{name}: {e}") from None
+    rc = getattr(_lib(), name)(packed, stream)
+    if rc:
+        raise DiagError(rc, name)
 
 
 def block_quantize_launch(src, dst, scales, rows, cols, dtype="bf16", blocks="rows", transpose=False, ld_src=0, ld_dst=0,
@@ -567,20 +564,16 @@ def block_quantize_launch(src, dst, scales, rows, cols, dtype="bf16", blocks="ro
     blocks="rows" (128 elements of a row; scales[ceil(c / 128)][r]) or "tiles" (128 x 128; scales[ceil(r / 128)][ceil(c / 128)]).
     scale = amax / 448 with amax at least 2^-96; rows of dst are padded to a multiple of 16 with zeros.  Device pointers as
     ints; strides in elements, 0 = packed."""
-    q = BlockQuantize(src, dst, scales, ld_src, ld_dst, ld_scales, rows, cols, DTYPES[dtype], BLOCKS[blocks], bool(transpose))
-    rc = _lib().gmd_block_quantize_launch(C.byref(q), stream)
-    if rc:
-        raise DiagError(rc, "gmd_block_quantize_launch")
+    _packed_launch("gmd_block_quantize_launch", _BLOCK_QUANTIZE, stream, src or 0, dst or 0, scales or 0, ld_src, ld_dst, ld_scales,
+                   rows, cols, DTYPES[dtype], BLOCKS[blocks], bool(transpose), 0)
 
 
 def gemm_block_launch(a, scale_a, b, scale_b, c, m, n, k, b_blocks="tiles", out="bf16", lda=0, ldb=0, ldc=0, ld_scale_a=0,
                       ld_scale_b=0, stream=None):
     """C[m, n] ("bf16" or "f32") = A[m, k] @ B[n, k]^T of e4m3 operands with an f32 scale per block of 128
     (block_quantize_launch): A's blocks are rows, B's tiles or rows.  Any m, n a multiple of 8, k of 16."""
-    g = GemmBlock(a, b, c, scale_a, scale_b, lda, ldb, ldc, ld_scale_a, ld_scale_b, m, n, k, BLOCKS[b_blocks], DTYPES[out])
-    rc = _lib().gmd_gemm_block_launch(C.byref(g), stream)
-    if rc:
-        raise DiagError(rc, "gmd_gemm_block_launch")
+    _packed_launch("gmd_gemm_block_launch", _GEMM_BLOCK, stream, a or 0, b or 0, c or 0, scale_a or 0, scale_b or 0, lda, ldb, ldc,
+                   ld_scale_a, ld_scale_b, m, n, k, BLOCKS[b_blocks], DTYPES[out], 0)
 
 
 def grouped_gemm_launch(op, dtype, a, b, c, offsets, groups, rows, n, k, out="bf16", scale_a=None, scale_b=None, lda=0, ldb=0,
@@ -589,8 +582,6 @@ def grouped_gemm_launch(op, dtype, a, b, c, offsets, groups, rows, n, k, out="bf
     "forward": c[rows, n] = a[rows, k] w[e]^T with b = w [groups][n, k]; "dgrad": c[rows, k] = a[rows, n] w[e];
     "wgrad": c[groups][n, k] = per expert a[rows, n]^T b[rows, k].  dtype "bf16", or "fp8" (forward; e4m3 in blocks of
     128 with scale_a per row and scale_b per tile of w).  Rows outside every expert's range are left as they were."""
-    g = GroupedGemm(a, b, c, offsets, scale_a, scale_b, lda, ldb, ldc, stride_w, ld_scale_a, ld_scale_b, stride_scale,
-                    GROUPED_OPS[op], DTYPES[dtype], DTYPES[out], groups, rows, n, k)
-    rc = _lib().gmd_grouped_gemm_launch(C.byref(g), stream)
-    if rc:
-        raise DiagError(rc, f"gmd_grouped_gemm_launch({op}, {dtype})")
+    _packed_launch("gmd_grouped_gemm_launch", _GROUPED_GEMM, stream, a or 0, b or 0, c or 0, offsets or 0, scale_a or 0, scale_b or 0,
+                   lda, ldb, ldc, stride_w, ld_scale_a, ld_scale_b, stride_scale, GROUPED_OPS[op], DTYPES[dtype], DTYPES[out],
+                   groups, rows, n, k, 0)

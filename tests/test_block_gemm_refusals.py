@@ -1,6 +1,10 @@
 """What the block-scaled fp8 and expert-grouped GEMM entry points refuse, before anything reaches a GPU (no GPU needed: the
 pointers are never followed)."""
 import os
+import re
+import shutil
+import struct
+import subprocess
 
 import pytest
 
@@ -39,6 +43,7 @@ def test_quantize_refusals(diag):
     refused(diag, "stride of scales", f, P, Q, R, 300, 200, ld_scales=299)
     refused(diag, "stride of scales", f, P, Q, R, 300, 200, blocks="tiles", ld_scales=1)
     refused(diag, "stride of scales", f, P, Q, R, 300, 200, blocks="tiles", transpose=True, ld_scales=2)
+    refused(diag, "gmd_block_quantize_launch", f, P, Q, R, 1 << 31, 8)          # does not fit its field
     with pytest.raises(KeyError):
         f(P, Q, R, 8, 8, blocks="columns")
     f(None, None, None, 0, 128)  # a size of zero is no error
@@ -103,3 +108,27 @@ def test_grouped_refusals(diag):
     f("forward", "bf16", None, None, None, None, 4, 0, 64, 64)
     f("forward", "bf16", None, None, None, None, 0, 100, 64, 64)
     f("wgrad", "bf16", None, None, None, None, 4, 100, 0, 64)
+
+
+def test_packed_structs_match_the_header(diag, tmp_path):
+    """Sizes and the offset of every field as a C compiler lays them out."""
+    if not shutil.which("g++"):
+        pytest.skip("needs a C++ compiler")
+    fields = {"gmd_block_quantize_t": (diag._BLOCK_QUANTIZE, "src dst scales ld_src ld_dst ld_scales rows cols src_dtype blocks transpose reserved"),
+              "gmd_gemm_block_t": (diag._GEMM_BLOCK, "a b c scale_a scale_b lda ldb ldc ld_scale_a ld_scale_b m n k b_blocks out_dtype reserved"),
+              "gmd_grouped_gemm_t": (diag._GROUPED_GEMM, "a b c offsets scale_a scale_b lda ldb ldc stride_w ld_scale_a ld_scale_b stride_scale op "
+                                     "dtype out_dtype groups rows n k reserved")}
+    src = '#include <cstdio>\n#include "gpumon_diag.h"\nint main() {\n'
+    for t, (_, names) in fields.items():
+        src += f'printf("%zu", sizeof({t}));\n' + "".join(f'printf(" %zu", __builtin_offsetof({t}, {n}));\n' for n in names.split()) + 'puts("");\n'
+    (tmp_path / "f.cc").write_text(src + "}\n")
+    subprocess.run(["g++", "-I", os.path.join(ROOT, "diag"), "-o", str(tmp_path / "f"), str(tmp_path / "f.cc")], check=True)
+    lines = subprocess.run([str(tmp_path / "f")], check=True, capture_output=True, text=True).stdout.splitlines()
+    import struct
+    for line, (form, names) in zip(lines, fields.values()):
+        size, *offsets = map(int, line.split())
+        assert form.size == size
+        flat = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([Pqi])", form.format))
+        assert len(flat) == len(names.split())
+        at = [struct.calcsize(flat[:i]) for i in range(len(flat))]
+        assert at == offsets
