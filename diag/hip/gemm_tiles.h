@@ -173,10 +173,13 @@ struct Stage {
 
   // Which KiB of the tile's image piece i of a wave is.
   static __device__ __forceinline__ int place(int wave, int i) {
-    if constexpr (HALVES == 0) return wave * kPieces + i;
-    constexpr int per = kPieces / 2, block = HALVES / 16;  // pieces per wave and half; KiB of one wave row's half
-    const int q = wave * per + i % per;                    // among the pieces of this half
-    return q / block * 2 * block + i / per * block + q % block;
+    if constexpr (HALVES == 0) {
+      return wave * kPieces + i;
+    } else {
+      constexpr int per = kPieces / 2, block = HALVES / 16;  // pieces per wave and half; KiB of one wave row's half
+      const int q = wave * per + i % per;                    // among the pieces of this half
+      return q / block * 2 * block + i / per * block + q % block;
+    }
   }
   // first: first row (column) of the tile, rows_left >= 1: how many of them exist; the rest repeat the last one.
   __device__ __forceinline__ void init(const char* p, int64_t ld_, int64_t first, int rows_left, int wave, int lane) {
@@ -343,7 +346,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   constexpr int kStrip = WTN * 4 + 16;  // epilogue: one row of a wave's strip of 16 rows
   static_assert(kWaves * 16 * kStrip <= 2 * kBufBytes, "the epilogue's strips fit into the operand buffers");
   constexpr int kScaleBytes = kFp8 ? kWaves * 256 : 0;
-  static_assert(BM / 64 + (KIND == kFp8Rows ? BN / 64 : 1) <= kWaves, "one DMA of scales per wave and step");
+  static_assert(!kFp8 || BM / 64 + (KIND == kFp8Rows ? BN / 64 : 1) <= kWaves, "one DMA of scales per wave and step");
   __shared__ __attribute__((aligned(16))) char smem[2 * (kBufBytes + kScaleBytes)];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -816,6 +819,8 @@ int launch_forward(const Args& p, hipStream_t st) {
   if (nb == 1) return launch_few<KIND, 4, 1, 6, 2, OUT>(p, st);
   if (nb == 2) return launch_few<KIND, 4, 2, 8, 1, OUT>(p, st);
   if (nb == 4) return launch_few<KIND, 4, 4, 4, 2, OUT>(p, st);
+  // up to two workgroups a CU, which one slot each leaves room for (203 x 4120 x 2064: 13.5 us, tiles 17.3; 512 x 3840 x 2048: 13.6 and 13.7)
+  if (grid_of(p, 64, 64) <= 2 * kCUs) return launch_few<KIND, 4, 4, 4, 1, OUT>(p, st);
   // (f32 results of e4m3 operands are computed on widened fragments, which do not fit the large tile's registers)
   if constexpr (KIND == kBf16 || sizeof(OUT) == 2)
     if (large_tiles(p, KIND == kBf16 ? 64 : 128)) return launch_tile<KIND, false, false, 256, 256, 2, 4, OUT>(p, st);
