@@ -30,6 +30,13 @@ def dev():
     return torch.device("cuda", 0)
 
 
+@pytest.fixture(scope="module", autouse=True)
+def memory_back():
+    """The largest cases take tens of GB; other tests measure bandwidth in processes of their own."""
+    yield
+    torch.cuda.empty_cache()
+
+
 def _stream():
     return torch.cuda.current_stream().cuda_stream
 
