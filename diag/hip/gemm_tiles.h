@@ -125,6 +125,21 @@ __device__ __forceinline__ bool find_tile(const Args& p, int bm, int bn, int id,
   return false;
 }
 
+// The weight gradient's tile of this workgroup, and its expert's rows as the contraction.  Every XCD takes an eighth of every
+// expert's tiles, neighbours of the walk: the experts' numbers of rows differ, and with them what a tile costs (16k rows over 16
+// experts of 4096 x 2048: 305 us, with whole experts dealt to the XCDs 470).
+__device__ __forceinline__ bool wgrad_tile(const Args& p, int bm, int bn, Tile* t, int64_t* k_first, int* K) {
+  const int tiles_m = (p.m + bm - 1) / bm, tiles_n = (p.n + bn - 1) / bn, eighth = (tiles_m * tiles_n + 7) / 8;
+  const int slot = (int)blockIdx.x >> 3, work = ((int)blockIdx.x & 7) * eighth + slot % eighth;
+  if (work >= tiles_m * tiles_n) return false;
+  int tm, tn, lo, hi;
+  tile_walk(work, tiles_m, tiles_n, &tm, &tn);
+  t->group = slot / eighth, t->m0 = tm * bm, t->m_end = p.m, t->n0 = tn * bn;
+  group_rows(p.offsets, t->group, p.k, &lo, &hi);
+  *k_first = lo, *K = hi - lo;
+  return true;
+}
+
 // ------------------------------------------------------------------------------------------------------ LDS image --
 // k contiguous: 8 rows x 128 bytes per KiB, which is what one wave-wide LDS-DMA instruction of 16 bytes a lane writes,
 // the 16-byte chunks of row r permuted by chunk ^ swizzle(r).  A fragment read (ds_read_b128, lane (fr, fq): row fr, chunk
@@ -138,10 +153,10 @@ __device__ __forceinline__ int chunk_swizzle(int row) { return ((row >> 1) & 3) 
 // unit ^ unit_swizzle(row) so that these eight units lie in different banks (64 banks of 4 bytes).  COLS: columns of the image.
 template <int COLS>
 __device__ __forceinline__ int unit_swizzle(int row) {
-  static_assert(COLS >= 32, "two units at least");
   if constexpr (COLS >= 128) return ((row >> 3) & 1) * 4 + (row & 3);
   if constexpr (COLS == 64) return ((row >> 3) & 1) * 2 + ((row >> 1) & 1);
-  return (row >> 3) & 1;
+  if constexpr (COLS == 32) return (row >> 3) & 1;
+  return 0;  // one unit a row
 }
 
 // One LDS-DMA instruction: SGPR base + 32-bit VGPR offset -> M0 + lane * BYTES.  Through the builtin every one costs a 64-bit
@@ -356,17 +371,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   int64_t k_first = 0;
   int K = p.k;
   if constexpr (WGRAD) {
-    // Every XCD takes an eighth of every expert's tiles, neighbours of the walk: the experts' numbers of rows differ, and with
-    // them what a tile costs (whole experts dealt to XCDs: GMD_WGRAD_BY_EXPERT us against GMD_WGRAD_EIGHTHS, 16k rows over 16 experts of 4096 x 2048).
-    const int tiles_m = (p.m + BM - 1) / BM, tiles_n = (p.n + BN - 1) / BN, eighth = (tiles_m * tiles_n + 7) / 8;
-    const int slot = (int)blockIdx.x >> 3, work = ((int)blockIdx.x & 7) * eighth + slot % eighth;
-    if (work >= tiles_m * tiles_n) return;
-    int tm, tn, lo, hi;
-    t.group = slot / eighth;
-    tile_walk(work, tiles_m, tiles_n, &tm, &tn);
-    t.m0 = tm * BM, t.m_end = p.m, t.n0 = tn * BN;
-    group_rows(p.offsets, t.group, p.k, &lo, &hi);
-    k_first = lo, K = hi - lo;
+    if (!wgrad_tile(p, BM, BN, &t, &k_first, &K)) return;
   } else {
     if (!find_tile(p, BM, BN, blockIdx.x, &t)) return;  // the whole workgroup, before any barrier
   }
@@ -615,34 +620,38 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
 // Through LDS and not straight into registers because of the address path: it takes a quad of lanes that asks for 64
 // contiguous bytes in one cycle, but lanes of an MFMA operand are neighbours in different rows, one lane a cycle (64 rows of
 // 512 x 8192 e4m3: GMD_US_DIRECT us loaded directly, GMD_US_LDS this way).
-template <int KIND, int MB, int NB, int W, int U, typename OUT>
+template <int KIND, bool TA, bool TB, int MB, int NB, int W, int U, typename OUT>
 __global__ __launch_bounds__(W * 64) void few_rows_kernel(Args p) {
-  constexpr bool kFp8 = KIND != kBf16, kNarrow = sizeof(OUT) == 2;
-  constexpr int kElem = kFp8 ? 1 : 2;
+  constexpr bool kFp8 = KIND != kBf16, kNarrow = sizeof(OUT) == 2, kWgrad = TA;
+  constexpr int kElem = kFp8 ? 1 : 2, kStepK = kStepBytes / kElem;
   constexpr int kPieces = 2 * (MB + NB), kScaleDmas = !kFp8 ? 0 : KIND == kFp8Rows ? 2 : 1, kDmas = kPieces + kScaleDmas;
   constexpr int kSlot = kPieces * 1024 + kScaleDmas * 256;
   static_assert(MB <= 4 && NB <= 4 && 128 % (NB * 16) == 0, "a step's scales in one DMA each, the columns inside one tile of scales");
   static_assert((U - 1) * kDmas < 64 && W * MB * NB * 1024 <= W * U * kSlot, "vmcnt counts to 63; the sums fit into the ring");
+  static_assert(!kFp8 || (!TA && !TB), "block-scaled fp8: k contiguous");
   __shared__ __attribute__((aligned(16))) char smem[W * U * kSlot];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Tile t;
-  if (!find_tile(p, MB * 16, NB * 16, blockIdx.x, &t)) return;
-  const int kbytes = p.k * kElem;
-  const int steps = (kbytes + kStepBytes - 1) / kStepBytes;
+  int64_t k_first = 0;
+  int K = p.k;
+  if constexpr (kWgrad) {
+    if (!wgrad_tile(p, MB * 16, NB * 16, &t, &k_first, &K)) return;
+  } else {
+    if (!find_tile(p, MB * 16, NB * 16, blockIdx.x, &t)) return;
+  }
+  const int steps = (int)(((int64_t)K + kStepK - 1) / kStepK), whole = K / kStepK;
   const int mine = steps > wave ? (steps - wave + W - 1) / W : 0;  // this wave's: wave, wave + W, ...
   char* const ring = smem + wave * U * kSlot;
 
-  // Piece i: rows 8 i .. 8 i + 7 of A and then of B, 128 bytes each; rows beyond the last repeat it.
-  const char* const a_base = p.a + (int64_t)t.m0 * p.lda;
-  const char* const b_base = p.b + t.group * p.stride_b + (int64_t)t.n0 * p.ldb;
-  uint32_t off[kPieces];
-  const int chunk = (lane & 7) ^ chunk_swizzle(lane >> 3);
-#pragma unroll
-  for (int i = 0; i < kPieces; i++) {
-    const int r = i * 8 + (lane >> 3);
-    off[i] = (uint32_t)(r < MB * 16 ? min(r, t.m_end - 1 - t.m0) * p.lda : min(r - MB * 16, p.n - 1 - t.n0) * p.ldb) + chunk * 16;
-  }
+  Stage<TA, MB * 16, 1, 0, false> ga;
+  Stage<TB, NB * 16, 1, 0, false> gb;
+  ga.init(p.a + (TA ? k_first * p.lda : 0), p.lda, t.m0, t.m_end - t.m0, 0, lane);
+  gb.init(p.b + (kWgrad ? 0 : t.group * p.stride_b) + (TB ? k_first * p.ldb : 0), p.ldb, t.n0, p.n - t.n0, 0, lane);
+  Frags<TA, MB * 16, MB, 0> fa;
+  Frags<TB, NB * 16, NB, 0> fb;
+  fa.init(0, lane);
+  fb.init(0, lane);
   const float* const sa_base = kFp8 ? p.sa + t.m0 : nullptr;
   const uint32_t sa_off = (uint32_t)min(lane, t.m_end - 1 - t.m0) * 4;
   const float* const SB = !kFp8 ? nullptr : p.sb + t.group * p.stride_sb + (KIND == kFp8Rows ? (int64_t)t.n0 : (int64_t)(t.n0 / 128) * p.ld_sb);
@@ -650,17 +659,19 @@ __global__ __launch_bounds__(W * 64) void few_rows_kernel(Args p) {
   auto issue = [&](int s) {
     const int kt = wave + s * W;
     char* const slot = ring + s % U * kSlot;
-    const char* const at_a = a_base + (int64_t)kt * kStepBytes;
-    const char* const at_b = b_base + (int64_t)kt * kStepBytes;
-    if ((kt + 1) * kStepBytes <= kbytes) {
+    if (kt < whole) {
+      const char* const at_a = ga.step_base(kt);
+      const char* const at_b = gb.step_base(kt);
 #pragma unroll
-      for (int i = 0; i < kPieces; i++) dma<16>(i < 2 * MB ? at_a : at_b, off[i], slot + i * 1024);
+      for (int i = 0; i < 2 * MB; i++) ga.fetch(at_a, slot, 0, i);
+#pragma unroll
+      for (int i = 0; i < 2 * NB; i++) gb.fetch(at_b, slot + MB * 2048, 0, i);
     } else {  // K ends inside this step: zeros behind it
-      const bool in = kt * kStepBytes + chunk * 16 < kbytes;
+      const int64_t left = (int64_t)K - (int64_t)kt * kStepK;
 #pragma unroll
-      for (int i = 0; i < kPieces; i++)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(in ? (i < 2 * MB ? at_a : at_b) + off[i] : (const char*)&g_zero16),
-                                         (__attribute__((address_space(3))) void*)(slot + i * 1024), 16, 0, 0);
+      for (int i = 0; i < 2 * MB; i++) ga.fetch_edge(ga.step_base(kt), TA ? left : left * kElem, slot, 0, i);
+#pragma unroll
+      for (int i = 0; i < 2 * NB; i++) gb.fetch_edge(gb.step_base(kt), TB ? left : left * kElem, slot + MB * 2048, 0, i);
     }
     if constexpr (kFp8) dma<4>(sa_base + kt * p.ld_sa, sa_off, slot + kPieces * 1024);
     if constexpr (KIND == kFp8Rows) dma<4>(SB + kt * p.ld_sb, sb_off, slot + kPieces * 1024 + 256);
@@ -670,9 +681,6 @@ __global__ __launch_bounds__(W * 64) void few_rows_kernel(Args p) {
   for (int i = 0; i < MB; i++)
 #pragma unroll
     for (int j = 0; j < NB; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Frags<false, 16, 1, 0> frag;
-  frag.init(0, lane);
-
 #pragma unroll
   for (int u = 0; u < U; u++)
     if (u < mine) issue(u);
@@ -684,9 +692,9 @@ __global__ __launch_bounds__(W * 64) void few_rows_kernel(Args p) {
     const char* const slot = ring + s % U * kSlot;
     Operand<kFp8 ? (kNarrow ? 1 : 2) : 0> af[MB], bf[NB];
 #pragma unroll
-    for (int j = 0; j < NB; j++) bf[j].set(frag.read(slot, MB + j, 0), frag.read(slot, MB + j, 1));
+    for (int j = 0; j < NB; j++) bf[j].set(fb.read(slot + MB * 2048, j, 0), fb.read(slot + MB * 2048, j, 1));
 #pragma unroll
-    for (int i = 0; i < MB; i++) af[i].set(frag.read(slot, i, 0), frag.read(slot, i, 1));
+    for (int i = 0; i < MB; i++) af[i].set(fa.read(slot, i, 0), fa.read(slot, i, 1));
     float sa[MB];
     f32x4 sb[KIND == kFp8Rows ? NB : 1];
     if constexpr (kFp8) {
@@ -732,7 +740,7 @@ __global__ __launch_bounds__(W * 64) void few_rows_kernel(Args p) {
     for (int w = 1; w < W; w++) v += sums[(w * MB * NB + q) * 64 + lane];
     const int r = t.m0 + q / NB * 16 + fr, col = t.n0 + q % NB * 16 + fq * 4;
     if (r < t.m_end && col < p.n) {
-      OUT* dst = (OUT*)p.c + r * p.ldc + col;
+      OUT* dst = (OUT*)p.c + (kWgrad ? t.group * p.stride_c : 0) + r * p.ldc + col;
       if constexpr (sizeof(OUT) == 2) *(bf16x4*)dst = __builtin_convertvector(v, bf16x4);
       else *(f32x4*)dst = v;
     }
@@ -745,6 +753,11 @@ inline int64_t grid_of(const Args& p, int bm, int bn) {
   const int64_t tiles_n = ((int64_t)p.n + bn - 1) / bn;
   const int64_t tiles_m = p.offsets ? (int64_t)p.m / bm + std::min(p.groups, p.m) : ((int64_t)p.m + bm - 1) / bm;
   return tiles_m * tiles_n;
+}
+inline int64_t grid_for(const Args& p, bool wgrad, int bm, int bn) {
+  if (!wgrad) return grid_of(p, bm, bn);
+  const int64_t tiles = (((int64_t)p.m + bm - 1) / bm) * (((int64_t)p.n + bn - 1) / bn);
+  return p.groups * ((tiles + 7) / 8 * 8);  // wgrad_tile
 }
 inline int launched(const char* what, int64_t grid) {
   if (grid <= 0 || grid > 0x7fffffff) {
@@ -784,19 +797,17 @@ inline bool large_tiles(const Args& p, int step_k) {
 
 template <int KIND, bool TA, bool TB, int BM, int BN, int WM, int WN, typename OUT>
 int launch_tile(const Args& p, hipStream_t st) {
-  constexpr bool kWgrad = TA;
-  const int64_t tiles = (((int64_t)p.m + BM - 1) / BM) * (((int64_t)p.n + BN - 1) / BN);
-  const int64_t grid = kWgrad ? p.groups * ((tiles + 7) / 8 * 8) : grid_of(p, BM, BN);
+  const int64_t grid = grid_for(p, TA, BM, BN);
   if (int rc = launched("GEMM", grid)) return rc;
-  tile_kernel<KIND, TA, TB, kWgrad, BM, BN, WM, WN, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
+  tile_kernel<KIND, TA, TB, TA, BM, BN, WM, WN, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
   GMD_HIP(hipGetLastError());
   return GMD_OK;
 }
-template <int KIND, int MB, int NB, int W, int U, typename OUT>
+template <int KIND, bool TA, bool TB, int MB, int NB, int W, int U, typename OUT>
 int launch_few(const Args& p, hipStream_t st) {
-  const int64_t grid = grid_of(p, MB * 16, NB * 16);
+  const int64_t grid = grid_for(p, TA, MB * 16, NB * 16);
   if (int rc = launched("GEMM", grid)) return rc;
-  few_rows_kernel<KIND, MB, NB, W, U, OUT><<<(unsigned)grid, W * 64, 0, st>>>(p);
+  few_rows_kernel<KIND, TA, TB, MB, NB, W, U, OUT><<<(unsigned)grid, W * 64, 0, st>>>(p);
   GMD_HIP(hipGetLastError());
   return GMD_OK;
 }
@@ -806,21 +817,21 @@ int launch_forward(const Args& p, hipStream_t st) {
   const int mb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   const int nb = grid_of(p, 16 * mb, 16) <= kCUs ? 1 : grid_of(p, 16 * mb, 32) <= kCUs ? 2 : grid_of(p, 16 * mb, 64) <= kCUs ? 4 : 0;
   if (mb == 1) {
-    if (nb == 1) return launch_few<KIND, 1, 1, 8, 2, OUT>(p, st);
+    if (nb == 1) return launch_few<KIND, false, false, 1, 1, 8, 2, OUT>(p, st);
     // (e4m3 experts: a slot less in flight leaves room for twice the workgroups, 128 experts of 2048 x 1024 for 128 rows 42 -> 34 us)
-    if (p.offsets) return KIND == kBf16 ? launch_few<KIND, 1, 2, 4, 2, OUT>(p, st) : launch_few<KIND, 1, 2, 4, 1, OUT>(p, st);
-    return nb == 2 ? launch_few<KIND, 1, 2, 4, 2, OUT>(p, st) : launch_few<KIND, 1, 4, 4, 2, OUT>(p, st);
+    if (p.offsets) return KIND == kBf16 ? launch_few<KIND, false, false, 1, 2, 4, 2, OUT>(p, st) : launch_few<KIND, false, false, 1, 2, 4, 1, OUT>(p, st);
+    return nb == 2 ? launch_few<KIND, false, false, 1, 2, 4, 2, OUT>(p, st) : launch_few<KIND, false, false, 1, 4, 4, 2, OUT>(p, st);
   }
   if (mb == 2) {
-    if (nb == 1) return launch_few<KIND, 2, 1, 8, 2, OUT>(p, st);
-    if (p.offsets) return launch_few<KIND, 2, 4, 4, 1, OUT>(p, st);
-    return nb == 2 ? launch_few<KIND, 2, 2, 4, 2, OUT>(p, st) : launch_few<KIND, 2, 4, 4, 2, OUT>(p, st);
+    if (nb == 1) return launch_few<KIND, false, false, 2, 1, 8, 2, OUT>(p, st);
+    if (p.offsets) return launch_few<KIND, false, false, 2, 4, 4, 1, OUT>(p, st);
+    return nb == 2 ? launch_few<KIND, false, false, 2, 2, 4, 2, OUT>(p, st) : launch_few<KIND, false, false, 2, 4, 4, 2, OUT>(p, st);
   }
-  if (nb == 1) return launch_few<KIND, 4, 1, 6, 2, OUT>(p, st);
-  if (nb == 2) return launch_few<KIND, 4, 2, 8, 1, OUT>(p, st);
-  if (nb == 4) return launch_few<KIND, 4, 4, 4, 2, OUT>(p, st);
+  if (nb == 1) return launch_few<KIND, false, false, 4, 1, 6, 2, OUT>(p, st);
+  if (nb == 2) return launch_few<KIND, false, false, 4, 2, 8, 1, OUT>(p, st);
+  if (nb == 4) return launch_few<KIND, false, false, 4, 4, 4, 2, OUT>(p, st);
   // up to two workgroups a CU, which one slot each leaves room for (203 x 4120 x 2064: 13.5 us, tiles 17.3; 512 x 3840 x 2048: 13.6 and 13.7)
-  if (grid_of(p, 64, 64) <= 2 * kCUs) return launch_few<KIND, 4, 4, 4, 1, OUT>(p, st);
+  if (grid_of(p, 64, 64) <= 2 * kCUs) return launch_few<KIND, false, false, 4, 4, 4, 1, OUT>(p, st);
   // (f32 results of e4m3 operands are computed on widened fragments, which do not fit the large tile's registers)
   if constexpr (KIND == kBf16 || sizeof(OUT) == 2)
     if (large_tiles(p, KIND == kBf16 ? 64 : 128)) return launch_tile<KIND, false, false, 256, 256, 2, 4, OUT>(p, st);

@@ -12,14 +12,21 @@ namespace {
 template <typename OUT>
 int launch_bf16(int op, const Args& p, hipStream_t st) {
   if (op == GMD_GROUPED_FORWARD) return launch_forward<kBf16, OUT>(p, st);
-  if (op == GMD_GROUPED_DGRAD)
+  if (op == GMD_GROUPED_DGRAD) {
+    // As in the forward, but always 64 columns a workgroup: a row of W is read in pieces of that many.
+    const int rows = (p.m + p.groups - 1) / p.groups;
+    if (rows <= 16) return launch_few<kBf16, false, true, 1, 4, 8, 1, OUT>(p, st);
+    if (rows <= 32) return launch_few<kBf16, false, true, 2, 4, 6, 1, OUT>(p, st);
+    if (grid_of(p, 64, 64) <= 2 * kCUs) return launch_few<kBf16, false, true, 4, 4, 4, 1, OUT>(p, st);
     return large_tiles(p, 64) ? launch_tile<kBf16, false, true, 256, 256, 2, 4, OUT>(p, st) : launch_tile<kBf16, false, true, 128, 128, 4, 2, OUT>(p, st);
+  }
+  if (grid_for(p, true, 64, 64) <= 2 * kCUs) return launch_few<kBf16, true, true, 4, 4, 4, 1, OUT>(p, st);
   Args one = p;  // an expert's share of the rows is its contraction
   one.offsets = nullptr, one.k = (p.k + p.groups - 1) / p.groups, one.m = p.m;
   const double steps = std::ceil(one.k / 64.0);
   return TileCost::large(p.groups * tiles_of(one, 256, 256), steps) < TileCost::small(p.groups * tiles_of(one, 128, 128), steps)
              ? launch_tile<kBf16, true, true, 256, 256, 2, 4, OUT>(p, st)
-             : launch_tile<kBf16, true, true, 128, 128, 2, 2, OUT>(p, st);
+             : launch_tile<kBf16, true, true, 128, 128, 4, 2, OUT>(p, st);
 }
 
 }  // namespace
