@@ -75,21 +75,15 @@ __device__ __forceinline__ void group_rows(const int* __restrict__ offsets, int 
   *hi = min(max(offsets[g + 1], *lo), rows);
 }
 
-// The tile that workgroup `id` of a launch over all experts' rows computes.  The host does not know the offsets, so the
-// grid is an upper bound (rows / bm + groups rows of tiles); ids beyond the real number return false.  Every wave scans
-// the tile counts, 64 experts at a time.
-__device__ __forceinline__ bool find_tile(const Args& p, int bm, int bn, int id, Tile* t) {
-  const int tiles_n = (p.n + bn - 1) / bn;
-  if (!p.offsets) {
-    const int tiles_m = (p.m + bm - 1) / bm;
-    int tm, tn;
-    tile_walk(xcd_contiguous(id, tiles_m * tiles_n), tiles_m, tiles_n, &tm, &tn);
-    t->group = 0, t->m0 = tm * bm, t->m_end = p.m, t->n0 = tn * bn;
-    return true;
-  }
-  const int lane = threadIdx.x & 63;
-  int lo = 0, hi = 0, upto = 0;  // of expert g0 + lane; tiles up to and with it, among these 64
-  auto scan = [&](int g0) {
+// The tiles of a launch over all experts' rows, in the order of the ids.  The host does not know the offsets, so its grid is an
+// upper bound (rows / bm + groups rows of tiles); ids beyond the real number have no tile.  Every wave scans the tile counts, 64
+// experts at a time, and keeps those of the last 64.
+struct RowTiles {
+  int bm, bn, tiles_n, total;
+  int lo, hi, upto;  // of expert g0 + lane; tiles up to and with it, among these 64
+
+  __device__ __forceinline__ void scan(const Args& p, int g0) {
+    const int lane = threadIdx.x & 63;
     lo = hi = 0;
     if (g0 + lane < p.groups) group_rows(p.offsets, g0 + lane, p.m, &lo, &hi);
     upto = (hi - lo + bm - 1) / bm * tiles_n;
@@ -98,39 +92,53 @@ __device__ __forceinline__ bool find_tile(const Args& p, int bm, int bn, int id,
       const int v = __shfl_up(upto, off, 64);
       if (lane >= off) upto += v;
     }
-  };
-  int total = 0;
-  for (int g0 = 0; g0 < p.groups; g0 += 64) {
-    scan(g0);
-    total += __builtin_amdgcn_readlane(upto, 63);
   }
-  if (id >= total) return false;
-  const int work = xcd_contiguous(id, total);
-  int before = 0;  // tiles of the experts in front
-  for (int g0 = 0; g0 < p.groups; g0 += 64) {
-    if (p.groups > 64) scan(g0);  // up to 64 are still there
-    const int in = work - before;
-    const unsigned long long has = __ballot(in < upto);
-    if (has) {
-      const int l = __builtin_ctzll(has);  // the first expert whose tiles reach past this one
-      const int glo = __builtin_amdgcn_readlane(lo, l), ghi = __builtin_amdgcn_readlane(hi, l);
-      const int tiles_m = (ghi - glo + bm - 1) / bm, first = __builtin_amdgcn_readlane(upto, l) - tiles_m * tiles_n;
-      int tm, tn;
-      tile_walk(in - first, tiles_m, tiles_n, &tm, &tn);
-      t->group = g0 + l, t->m0 = glo + tm * bm, t->m_end = ghi, t->n0 = tn * bn;
+  __device__ __forceinline__ void init(const Args& p, int bm_, int bn_) {
+    bm = bm_, bn = bn_, tiles_n = (p.n + bn - 1) / bn;
+    if (!p.offsets) {
+      total = (p.m + bm - 1) / bm * tiles_n;
+      return;
+    }
+    total = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += 64) {
+      scan(p, g0);
+      total += __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+  __device__ __forceinline__ bool find(const Args& p, int id, Tile* t) {
+    if (id >= total) return false;
+    const int work = xcd_contiguous(id, total);
+    int tm, tn;
+    if (!p.offsets) {
+      tile_walk(work, (p.m + bm - 1) / bm, tiles_n, &tm, &tn);
+      t->group = 0, t->m0 = tm * bm, t->m_end = p.m, t->n0 = tn * bn;
       return true;
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    int before = 0;  // tiles of the experts in front
+    for (int g0 = 0; g0 < p.groups; g0 += 64) {
+      if (p.groups > 64) scan(p, g0);  // up to 64 are still there
+      const int in = work - before;
+      const unsigned long long has = __ballot(in < upto);
+      if (has) {
+        const int l = __builtin_ctzll(has);  // the first expert whose tiles reach past this one
+        const int glo = __builtin_amdgcn_readlane(lo, l), ghi = __builtin_amdgcn_readlane(hi, l);
+        const int tiles_m = (ghi - glo + bm - 1) / bm, first = __builtin_amdgcn_readlane(upto, l) - tiles_m * tiles_n;
+        tile_walk(in - first, tiles_m, tiles_n, &tm, &tn);
+        t->group = g0 + l, t->m0 = glo + tm * bm, t->m_end = ghi, t->n0 = tn * bn;
+        return true;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
   }
-  return false;
-}
+};
 
-// The weight gradient's tile of this workgroup, and its expert's rows as the contraction.  Every XCD takes an eighth of every
+// The weight gradient's tile with this id, and its expert's rows as the contraction.  Every XCD takes an eighth of every
 // expert's tiles, neighbours of the walk: the experts' numbers of rows differ, and with them what a tile costs (16k rows over 16
 // experts of 4096 x 2048: 305 us, with whole experts dealt to the XCDs 470).
-__device__ __forceinline__ bool wgrad_tile(const Args& p, int bm, int bn, Tile* t, int64_t* k_first, int* K) {
+__device__ __forceinline__ bool wgrad_tile(const Args& p, int bm, int bn, int id, Tile* t, int64_t* k_first, int* K) {
   const int tiles_m = (p.m + bm - 1) / bm, tiles_n = (p.n + bn - 1) / bn, eighth = (tiles_m * tiles_n + 7) / 8;
-  const int slot = (int)blockIdx.x >> 3, work = ((int)blockIdx.x & 7) * eighth + slot % eighth;
+  const int slot = id >> 3, work = (id & 7) * eighth + slot % eighth;
   if (work >= tiles_m * tiles_n) return false;
   int tm, tn, lo, hi;
   tile_walk(work, tiles_m, tiles_n, &tm, &tn);
@@ -183,7 +191,6 @@ struct Stage {
   static constexpr int kChunks = kCols / 8;                 // ... and 16-byte chunks of its rows, which is also its size in KiB
   const char* base;        // first row of the tile, first k
   uint32_t off[kPieces];   // a lane's place in it
-  int chunk[kPieces];      // its chunk of the 128 bytes (k contiguous) or its row of the 64 (transposed)
   int64_t ld;
 
   // Which KiB of the tile's image piece i of a wave is.
@@ -208,14 +215,12 @@ struct Stage {
         const int c = (pos % kChunks) ^ (2 * unit_swizzle<kCols>(r));
         const int col = min(image * kCols + c * 8, rows_left - 8);  // the extent is a multiple of 8
         off[i] = (uint32_t)(r * ld) + (uint32_t)col * 2;
-        chunk[i] = r;
       } else {
         const int l = piece * 8 + (lane >> 3);
         int row = l;
         if constexpr (DEAL) row = l / HALVES * HALVES + (l & 15) * (HALVES / 16) + (l % HALVES >> 4);
         const int c = (lane & 7) ^ chunk_swizzle(l);
         off[i] = (uint32_t)(min(row, rows_left - 1) * ld) + (uint32_t)c * 16;
-        chunk[i] = c;
       }
     }
   }
@@ -228,7 +233,9 @@ struct Stage {
   }
   // Piece i of any K-step; `left` = k (elements if transposed, bytes if not) from this step on: what lies beyond is zero.
   __device__ __forceinline__ void fetch_edge(const char* src, int64_t left, char* tile, int wave, int i) const {
-    const bool in = TRANS ? chunk[i] < left : chunk[i] * 16 < left;
+    const int lane = threadIdx.x & 63;
+    const int at = TRANS ? (place(wave, i) % kChunks * 64 + lane) / kChunks : ((lane & 7) ^ chunk_swizzle(lane >> 3)) * 16;  // its row or byte of k
+    const bool in = at < left;
     const char* const from = in ? src + off[i] : (const char*)&g_zero16;
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                      (__attribute__((address_space(3))) void*)(tile + place(wave, i) * 1024), 16, 0, 0);
@@ -327,22 +334,6 @@ struct Operand<2> {
   }
 };
 
-// 16 bytes of a row of C, eight bf16 or four f32.  (Stored past the caches: no difference, 32k x 4096 x 2048 bf16 over 32 experts.)
-template <typename OUT>
-__device__ __forceinline__ void store16(OUT* dst, const char* f32s) {
-  u32x4 o;
-  if constexpr (sizeof(OUT) == 2) {
-    const f32x4 x = *(const f32x4*)f32s, y = *(const f32x4*)(f32s + 16);
-    o[0] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{x[0], x[1]}, bf16x2));
-    o[1] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{x[2], x[3]}, bf16x2));
-    o[2] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{y[0], y[1]}, bf16x2));
-    o[3] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{y[2], y[3]}, bf16x2));
-  } else {
-    o = *(const u32x4*)f32s;
-  }
-  *(u32x4*)dst = o;
-}
-
 // ------------------------------------------------------------------------------------------------------ tile kernel --
 // BM x BN of C per workgroup, WM x WN waves, K-steps double buffered in LDS: the next step's DMA is issued before this one
 // is computed on, one barrier per step.  The MFMA takes B's fragment first, so lane (fr, fq) of a 16 x 16 block holds row fr
@@ -351,56 +342,63 @@ __device__ __forceinline__ void store16(OUT* dst, const char* f32s) {
 // Block-scaled fp8: the matrix instruction sums one block of 128 k from zero and its result is added with one FMA per
 // element, acc += (sa * sb) * block.  With rows dealt to lanes (Stage's DEAL) a lane's scales of A are MB consecutive floats
 // per K-step, and B's tile scale is one scalar per wave.
-template <int KIND, bool TA, bool TB, bool WGRAD, int BM, int BN, int WM, int WN, typename OUT>
+template <int KIND, bool TA, bool TB, bool WGRAD, int BM, int BN, int WM, int WN, bool MANY, typename OUT>
 __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   constexpr int kWaves = WM * WN, WTM = BM / WM, WTN = BN / WN, MB = WTM / 16, NB = WTN / 16;
   constexpr bool kFp8 = KIND != kBf16, kNarrow = sizeof(OUT) == 2;
   constexpr int kElem = kFp8 ? 1 : 2, kStepK = kStepBytes / kElem;
   static_assert(!kFp8 || (!TA && !TB && WTN <= 128), "block-scaled fp8: k contiguous, a wave's columns inside one tile of scales");
   constexpr int kABytes = BM * kStepBytes, kBufBytes = (BM + BN) * kStepBytes;
-  constexpr int kStrip = WTN * 4 + 16;  // epilogue: one row of a wave's strip of 16 rows
-  static_assert(kWaves * 16 * kStrip <= 2 * kBufBytes, "the epilogue's strips fit into the operand buffers");
+  constexpr int kStripRows = kNarrow ? 16 : 8, kStrip = WTN * (int)sizeof(OUT) + 16, kStripBytes = kStripRows * kStrip;  // epilogue, per wave
+  static_assert(kWaves * kStripBytes <= 2 * kBufBytes, "the epilogue's strips fit into the operand buffers");
   constexpr int kScaleBytes = kFp8 ? kWaves * 256 : 0;
   static_assert(!kFp8 || BM / 64 + (KIND == kFp8Rows ? BN / 64 : 1) <= kWaves, "one DMA of scales per wave and step");
-  __shared__ __attribute__((aligned(16))) char smem[2 * (kBufBytes + kScaleBytes)];
+  __shared__ __attribute__((aligned(16))) char smem[2 * (kBufBytes + kScaleBytes) + (MANY ? kWaves * kStripBytes : 0)];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
-  Tile t;
+  // The tile at hand; MANY: ids blockIdx.x, blockIdx.x + gridDim.x, ...
+  Tile t{0, 0, 0, 0};
   int64_t k_first = 0;
   int K = p.k;
-  if constexpr (WGRAD) {
-    if (!wgrad_tile(p, BM, BN, &t, &k_first, &K)) return;
-  } else {
-    if (!find_tile(p, BM, BN, blockIdx.x, &t)) return;  // the whole workgroup, before any barrier
-  }
-  const char* const B = p.b + (WGRAD ? 0 : t.group * p.stride_b);
+  RowTiles tiles;
+  const int ids = WGRAD ? p.groups * (((p.m + BM - 1) / BM * ((p.n + BN - 1) / BN) + 7) / 8 * 8) : 0;
+  if constexpr (!WGRAD) tiles.init(p, BM, BN);
+  int id = blockIdx.x;
+  auto locate = [&]() {
+    bool found = false;
+    if constexpr (WGRAD) {
+      for (; id < ids && !found; id += found ? 0 : gridDim.x) found = wgrad_tile(p, BM, BN, id, &t, &k_first, &K);
+    } else {
+      found = tiles.find(p, id, &t);
+    }
+    // (uniform as they are; said so, the compiler keeps them, and the DMA's base addresses, in scalar registers across the loop)
+    t.group = __builtin_amdgcn_readfirstlane(t.group), t.m0 = __builtin_amdgcn_readfirstlane(t.m0);
+    t.m_end = __builtin_amdgcn_readfirstlane(t.m_end), t.n0 = __builtin_amdgcn_readfirstlane(t.n0);
+    k_first = __builtin_amdgcn_readfirstlane((int)k_first), K = __builtin_amdgcn_readfirstlane(K);
+    return (bool)__builtin_amdgcn_readfirstlane(found);
+  };
+  if (!locate()) return;  // the whole workgroup, before any barrier
   typedef Stage<TA, BM, kWaves, WTM, kFp8> StageA;
   typedef Stage<TB, BN, kWaves, 0, false> StageB;
   StageA ga;
   StageB gb;
-  ga.init(p.a + (TA ? k_first * p.lda : 0), p.lda, t.m0, t.m_end - t.m0, wave, lane);
-  gb.init(B + (TB ? k_first * p.ldb : 0), p.ldb, t.n0, p.n - t.n0, wave, lane);
   Frags<TA, BM, MB, WTM> fa;
   Frags<TB, BN, NB, 0> fb;
   fa.init(wm * WTM, lane);
   fb.init(wn * WTN, lane);
 
   f32x4 acc[MB][NB];
-#pragma unroll
-  for (int i = 0; i < MB; i++)
-#pragma unroll
-    for (int j = 0; j < NB; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // Scales of one K-step travel with its operands: A's of the tile's rows and B's of its columns (or of its 128-column
   // tiles) in a slot of their own behind the operand buffers, one DMA of 4 bytes a lane for 64 of them.  Loaded by each wave for
   // itself into registers they cost more than the matrix work: nine loads of their own per lane, wave and step.
-  const float* const SB = kFp8 ? p.sb + t.group * p.stride_sb : nullptr;
   const float* scale_src = nullptr;  // at step 0, this wave's part
   uint32_t scale_off = 0;            // this lane's place in it
   int64_t scale_ld = 0;
-  if constexpr (kFp8) {
+  auto scales_of_tile = [&](int lane) {
+    const float* const SB = p.sb + t.group * p.stride_sb;
     if (wave < BM / 64) {
       const int row = t.m0 + wave * 64;
       scale_src = p.sa + min(row, t.m_end - 1), scale_ld = p.ld_sa;
@@ -413,7 +411,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
       scale_src = SB + (int64_t)(t.n0 / 128) * p.ld_sb, scale_ld = 1;
       scale_off = (uint32_t)(min(min(lane, BN / 128 - 1), (p.n - 1) / 128 - t.n0 / 128) * p.ld_sb * 4);
     }
-  }
+  };
   auto fetch_scales = [&](int kt) {
     dma<4>(scale_src + kt * scale_ld, scale_off, smem + 2 * kBufBytes + (kt & 1) * kScaleBytes + wave * 256);
   };
@@ -439,8 +437,15 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
     for (int i = 0; i < MB; i++) sl[i] *= sb[0][0];
   };
 
-  const int steps = (int)(((int64_t)K + kStepK - 1) / kStepK);
-  const int whole = K / kStepK;  // steps that lie inside k
+  int steps = 0, whole = 0;  // K-steps; those that lie inside k
+  auto prepare = [&]() {
+    int own = lane;
+    asm volatile("" : "+v"(own));  // as in store_tile
+    ga.init(p.a + (TA ? k_first * p.lda : 0), p.lda, t.m0, t.m_end - t.m0, wave, own);
+    gb.init(p.b + (WGRAD ? 0 : t.group * p.stride_b) + (TB ? k_first * p.ldb : 0), p.ldb, t.n0, p.n - t.n0, wave, own);
+    if constexpr (kFp8) scales_of_tile(own);
+    steps = (int)(((int64_t)K + kStepK - 1) / kStepK), whole = K / kStepK;
+  };
   // The DMAs of one step and wave in the order they are issued: B, the first half of A, the scales (the first kFirst), and
   // the second half of A (kSecond).
   constexpr int kHalfA = StageA::kPieces / 2, kFirst = StageB::kPieces + kHalfA + (kFp8 ? 1 : 0), kSecond = kHalfA;
@@ -492,24 +497,27 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
       acc[i][j][r] = __builtin_fmaf(KIND == kFp8Tiles ? s : s * sb[KIND == kFp8Tiles ? 0 : j][r], part[at & 3][r], acc[i][j][r]);
     asm volatile("" : "+v"(acc[i][j]));  // here, between the MFMAs: left to itself the compiler sinks all of them behind the last
   };
-  // vmcnt(behind) lgkmcnt(0) and a barrier; `behind`: DMAs that may stay in flight.
-  auto sync = [&](auto behind) {
-    constexpr int n = decltype(behind)::value;
-    __builtin_amdgcn_s_waitcnt((n & 15) | 0x70 | (n >> 4) << 14);
+  // vmcnt(behind) lgkmcnt(0) and a barrier; `behind`: DMAs that may stay in flight, and with `stored` the stores of the tile before.
+  constexpr int kStores = MB * 16 * (int)sizeof(OUT) / 16 * (WTN / 4) / 16;
+  bool after_stores = false;  // exactly kStores of them were issued behind the DMAs of steps 0 and 1
+  auto sync = [&](auto behind, bool stored = false) {
+    constexpr int n = decltype(behind)::value, m = n + kStores;
+    static_assert(!MANY || m < 64, "vmcnt counts to 63");
+    if (MANY && stored) __builtin_amdgcn_s_waitcnt((m & 15) | 0x70 | (m >> 4) << 14);
+    else __builtin_amdgcn_s_waitcnt((n & 15) | 0x70 | (n >> 4) << 14);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
   const std::integral_constant<int, 0> none;
   const std::integral_constant<int, kFirst + kSecond> step_behind;
-  if (steps > 0) {
-    fetch_edge(0, 0, kFirst + kSecond);
-    if (steps > 1) {
-      fetch_edge(1, 0, kFirst + kSecond);
-      sync(std::integral_constant<int, kFirst + 2 * kSecond>());
-    } else {
-      sync(none);
-    }
+  auto begin = [&]() {
+    if (steps > 0) fetch_edge(0, 0, kFirst + kSecond);
+    if (steps > 1) fetch_edge(1, 0, kFirst + kSecond);
+  };
+  auto first_fragments = [&]() {
+    if (steps > 1) sync(std::integral_constant<int, kFirst + 2 * kSecond>(), after_stores);
+    else sync(none);
 #pragma unroll
     for (int j = 0; j < NB; j++) {
       bf[j].set(fb.read(smem + kABytes, j, 0), fb.read(smem + kABytes, j, 1));
@@ -522,7 +530,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
       for (int i = 0; i < 4; i++) part[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       s_tail[0] = s_tail[1] = 0.f;
     }
-  }
+  };
   // FULL: step kt + 2 exists and lies inside k.
   auto step = [&](int kt, auto FULL) {
     constexpr bool kFull = decltype(FULL)::value;
@@ -536,13 +544,13 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
     for (int at = 0; at < kProducts; at++) {
       const int i = row_of(at), j = col_of(at);
       if (at == kMid) {
-        if (more) sync(step_behind);
+        if (more) sync(step_behind, after_stores && kt <= 1);
         else sync(none);
         if (!kFull && more2) fetch_edge(kt + 2, 0, kFirst);
       }
       if (at % NB == 0 && at <= kTail) af[(i + 1) & 1].set(fa.read(la, i + 1, 0), fa.read(la, i + 1, 1));
       if (at == kBar) {
-        if (more2) sync(step_behind);
+        if (more2) sync(step_behind, after_stores && kt == 0);
         else sync(none);
         if (!kFull && more2) fetch_edge(kt + 2, kFirst, kFirst + kSecond);
         if constexpr (KIND == kFp8Tiles) {
@@ -578,37 +586,88 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
       read_scales(kt + 1);
     }
   };
-  int kt = 0;
-  for (; kt + 2 < whole; kt++) step(kt, std::true_type());
-  for (; kt < steps; kt++) step(kt, std::false_type());
-  if constexpr (KIND == kFp8Tiles) {
-    if (steps > 0) {
-      add(kProducts - 2);
-      add(kProducts - 1);
-    }
-  }
-  __syncthreads();  // every wave is done with the operand buffers
-
-  // Epilogue: 16 rows of the wave's tile at a time through a strip of LDS of its own, so that neighbouring lanes store
+  // Epilogue: kStripRows rows of a wave's tile at a time through a strip of LDS of its own, so that neighbouring lanes store
   // neighbouring columns of one row.
-  char* const strip = smem + wave * 16 * kStrip;
-  OUT* const C = (OUT*)p.c + (WGRAD ? t.group * p.stride_c : 0);
   constexpr int kCols16 = 16 / (int)sizeof(OUT);  // columns of a 16-byte store
   constexpr int kLanesPerRow = WTN / kCols16, kRowsPerPass = 64 / kLanesPerRow;
+  char* const strip = smem + (MANY ? 2 * (kBufBytes + kScaleBytes) : 0) + wave * kStripBytes;
+  auto store_tile = [&](const Tile& o, auto FULL) {
+    int own = lane;
+    asm volatile("" : "+v"(own));  // what follows from the lane is worked out here and not kept in registers across the K loop
+    const int strip_row = own / kLanesPerRow, strip_col = own % kLanesPerRow * kCols16, fr = own & 15, fq = own >> 4;
+    constexpr int kApart = kFp8 ? MB : 1;  // rows of C between rows of the strip
+    const uint32_t off = (uint32_t)((strip_row * kApart * p.ldc + strip_col) * (int)sizeof(OUT));
+    OUT* const base = (OUT*)p.c + (WGRAD ? o.group * p.stride_c : 0) + (int64_t)(o.m0 + wm * WTM) * p.ldc + o.n0 + wn * WTN;
+    const bool col_in = o.n0 + wn * WTN + strip_col < p.n;  // N is a multiple of 8
 #pragma unroll
-  for (int i = 0; i < MB; i++) {
+    for (int i = 0; i < MB; i++) {
 #pragma unroll
-    for (int j = 0; j < NB; j++) *(f32x4*)(strip + fr * kStrip + (j * 16 + fq * 4) * 4) = acc[i][j];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+      for (int h = 0; h < 16 / kStripRows; h++) {
+        if (kNarrow || fr / kStripRows == h) {
 #pragma unroll
-    for (int r0 = 0; r0 < 16; r0 += kRowsPerPass) {
-      const int f = r0 + lane / kLanesPerRow, c = lane % kLanesPerRow * kCols16;
-      const int row = t.m0 + wm * WTM + (kFp8 ? f * MB + i : i * 16 + f), col = t.n0 + wn * WTN + c;
-      if (row < t.m_end && col < p.n) store16<OUT>(C + row * p.ldc + col, strip + f * kStrip + c * 4);  // N is a multiple of 8
+          for (int j = 0; j < NB; j++) {
+            OUT* const to = (OUT*)(strip + fr % kStripRows * kStrip) + j * 16 + fq * 4;
+            if constexpr (kNarrow) *(bf16x4*)to = __builtin_convertvector(acc[i][j], bf16x4);
+            else *(f32x4*)to = acc[i][j];
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r0 = 0; r0 < kStripRows; r0 += kRowsPerPass) {
+          const int row = kFp8 ? (h * kStripRows + r0) * MB + i : i * 16 + h * kStripRows + r0;  // of the pass's first strip row
+          char* const to = (char*)(base + row * p.ldc);
+          const u32x4 v = *(const u32x4*)(strip + (r0 + strip_row) * kStrip + strip_col * (int)sizeof(OUT));
+          if constexpr (decltype(FULL)::value) {
+            // As asm, so that there are exactly kStores of them for the counted waits (and the wait state that a wide store's data
+            // needs).  Past the caches, which would not keep a result of that many tiles (8192^3 bf16 dgrad 764 -> 728 us).
+            asm volatile("global_store_dwordx4 %0, %1, %2 nt\n\ts_nop 1" ::"v"(off), "v"(v), "s"(to) : "memory");
+          } else if (o.m0 + wm * WTM + row + strip_row * kApart < o.m_end && col_in) {
+            *(u32x4*)(to + off) = v;
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+  };
+
+  prepare();
+  begin();
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < MB; i++)
+#pragma unroll
+      for (int j = 0; j < NB; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (steps > 0) first_fragments();
+    int kt = 0;
+    for (; kt + 2 < whole; kt++) step(kt, std::true_type());
+    for (; kt < steps; kt++) step(kt, std::false_type());
+    if constexpr (KIND == kFp8Tiles) {
+      if (steps > 0) {
+        add(kProducts - 2);
+        add(kProducts - 1);
+      }
+    }
+    // Since the last kBar nothing but registers is needed of this tile's operands, so the next tile's first steps are on
+    // their way while this one is stored (and its stores while the next one is computed on).
+    const Tile o = t;
+    bool next = false;
+    if constexpr (MANY) {
+      id += gridDim.x;
+      next = locate();
+      if (next) {
+        prepare();
+        begin();
+      }
+    } else {
+      __syncthreads();  // the strips lie in the operand buffers: every wave is done with them
+    }
+    const bool full = MANY && o.m0 + BM <= o.m_end && o.n0 + BN <= p.n;
+    if (full) store_tile(o, std::integral_constant<bool, MANY>());
+    else store_tile(o, std::false_type());
+    if (!next) break;
+    after_stores = full;
   }
 }
 
@@ -636,9 +695,11 @@ __global__ __launch_bounds__(W * 64) void few_rows_kernel(Args p) {
   int64_t k_first = 0;
   int K = p.k;
   if constexpr (kWgrad) {
-    if (!wgrad_tile(p, MB * 16, NB * 16, &t, &k_first, &K)) return;
+    if (!wgrad_tile(p, MB * 16, NB * 16, blockIdx.x, &t, &k_first, &K)) return;
   } else {
-    if (!find_tile(p, MB * 16, NB * 16, blockIdx.x, &t)) return;
+    RowTiles tiles;
+    tiles.init(p, MB * 16, NB * 16);
+    if (!tiles.find(p, blockIdx.x, &t)) return;
   }
   const int steps = (int)(((int64_t)K + kStepK - 1) / kStepK), whole = K / kStepK;
   const int mine = steps > wave ? (steps - wave + W - 1) / W : 0;  // this wave's: wave, wave + W, ...
@@ -797,9 +858,13 @@ inline bool large_tiles(const Args& p, int step_k) {
 
 template <int KIND, bool TA, bool TB, int BM, int BN, int WM, int WN, typename OUT>
 int launch_tile(const Args& p, hipStream_t st) {
-  const int64_t grid = grid_for(p, TA, BM, BN);
+  int64_t grid = grid_for(p, TA, BM, BN);
   if (int rc = launched("GEMM", grid)) return rc;
-  tile_kernel<KIND, TA, TB, TA, BM, BN, WM, WN, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
+  // One large tile fits a CU: that many workgroups walk the tiles.  Not for the weight gradient, whose tiles cost what their experts
+  // have of rows: dealt out one by one as CUs come free they take 302 us, in fixed turns 368 (16k rows, 16 experts of 4096 x 2048).
+  constexpr bool kMany = BM * BN >= 256 * 256 && !TA;
+  if (kMany) grid = std::min<int64_t>(grid, kCUs);
+  tile_kernel<KIND, TA, TB, TA, BM, BN, WM, WN, kMany, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
   GMD_HIP(hipGetLastError());
   return GMD_OK;
 }
