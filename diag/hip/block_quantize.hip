@@ -6,6 +6,8 @@
 // and every product that reads it becomes NaN.
 #include "diag_common.h"
 
+#include <type_traits>
+
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -28,38 +30,48 @@ struct QuantArgs {
   float* scales;
   int64_t ld_src, ld_dst, ld_scales;  // elements
   int rows, cols;                     // of src
-  int vec;                            // src rows can be read in 16-byte pieces
   int stream;                         // the result is stored past the caches
 };
 
-// Eight consecutive elements of a row as f32; zeros outside the matrix.
+// Sixteen bytes at any element's address: rows of an odd length are read in the same pieces as others.  8192 x 4100 bf16,
+// rows: 23.2 us, with single elements for rows that do not begin at 16 bytes 48.5.
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+
+// Eight consecutive elements of a row, held as they are read (four registers of bf16) and widened where they are used; zeros
+// outside the matrix.
 template <typename SRC>
-__device__ __forceinline__ void load8(const QuantArgs& p, int row, int col, float (&x)[8]) {
+struct Eight {
+  typename std::conditional<sizeof(SRC) == 2, u32x4, f32x4[2]>::type v;
+  __device__ __forceinline__ float operator[](int j) const {
+    if constexpr (sizeof(SRC) == 2) return __builtin_bit_cast(float, j & 1 ? v[j / 2] & 0xffff0000u : v[j / 2] << 16);
+    else return v[j / 4][j % 4];
+  }
+};
+template <typename SRC>
+__device__ __forceinline__ Eight<SRC> load8(const QuantArgs& p, int row, int col) {
   const SRC* s = (const SRC*)p.src + (int64_t)row * p.ld_src + col;
-  if (row < p.rows && p.vec && col + 8 <= p.cols) {
-    if constexpr (sizeof(SRC) == 2) {
-      const u32x4 v = *(const u32x4*)s;
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        x[2 * j] = __builtin_bit_cast(float, v[j] << 16);
-        x[2 * j + 1] = __builtin_bit_cast(float, v[j] & 0xffff0000u);
-      }
-    } else {
-      const f32x4 v = *(const f32x4*)s, w = *(const f32x4*)(s + 4);
-#pragma unroll
-      for (int j = 0; j < 4; j++) x[j] = v[j], x[4 + j] = w[j];
-    }
+  Eight<SRC> x;
+  if (row < p.rows && col + 8 <= p.cols) {
+    if constexpr (sizeof(SRC) == 2) x.v = *(const u32x4_any*)s;
+    else x.v[0] = *(const f32x4_any*)s, x.v[1] = *(const f32x4_any*)(s + 4);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = row < p.rows && col + j < p.cols ? (float)s[j] : 0.f;
+    for (int j = 0; j < 8; j++) {
+      const SRC e = row < p.rows && col + j < p.cols ? s[j] : (SRC)0.f;
+      if constexpr (sizeof(SRC) == 2) x.v[j / 2] = j & 1 ? x.v[j / 2] | (unsigned)__builtin_bit_cast(uint16_t, e) << 16 : __builtin_bit_cast(uint16_t, e);
+      else x.v[j / 4][j % 4] = e;
+    }
   }
+  return x;
 }
 template <typename T>
 __device__ __forceinline__ void store(const QuantArgs& p, uint8_t* to, const T& v) {
   if (p.stream) __builtin_nontemporal_store(v, (T*)to);
   else *(T*)to = v;
 }
-__device__ __forceinline__ unsigned magnitude8(const float (&x)[8]) {
+template <typename SRC>
+__device__ __forceinline__ unsigned magnitude8(const Eight<SRC>& x) {
   unsigned m = 0;
 #pragma unroll
   for (int j = 0; j < 8; j++) m = max(m, magnitude(x[j]));
@@ -70,10 +82,10 @@ __device__ __forceinline__ unsigned e4m3x4(float a, float b, float c, float d) {
   return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
 }
 
-// Blocks of a row, not transposed: a wave takes 512 columns (four blocks, sixteen lanes each) of four rows, all loads in
+// Blocks of a row, not transposed: a wave takes 512 columns (four blocks, sixteen lanes each) of two rows, all loads in
 // flight before the first is used.  Memory-bound: reads of 1 KiB (bf16) and writes of 512 bytes per wave and row.
-// 16384 x 7168 bf16 in 56.3 us, 6.3 TB/s (eight rows per wave 58.6 us, sixteen 116; 128 x 128 regions 75.6 us).
-constexpr int kRowsWave = 4, kRowsGroup = 16, kColsGroup = 512;
+// 16384 x 7168 bf16 from memory in 63.7 us, 5.5 TB/s (one row per wave 67.9 us, four 68.9, eight 73.4).
+constexpr int kRowsWave = 2, kRowsGroup = 8, kColsGroup = 512;
 template <typename SRC>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs p) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -81,9 +93,9 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs p) {
   const int row0 = (int)blockIdx.x / groups_c * kRowsGroup + wave * kRowsWave;
   const int col = (int)blockIdx.x % groups_c * kColsGroup + lane * 8;
   if (row0 >= p.rows) return;
-  float x[kRowsWave][8];
+  Eight<SRC> x[kRowsWave];
 #pragma unroll
-  for (int i = 0; i < kRowsWave; i++) load8<SRC>(p, row0 + i, col, x[i]);
+  for (int i = 0; i < kRowsWave; i++) x[i] = load8<SRC>(p, row0 + i, col);
   const int last16 = (p.cols + 15) & ~15;
   float scale[kRowsWave];
 #pragma unroll
@@ -115,6 +127,9 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs p) {
 // workgroup, and four rows of a column pack into one dword of the transposed image.  In that image (128 bytes per column)
 // the 16-byte chunks of a column are permuted by chunk ^ (column / 8), which leaves the dword writes at two per bank and the
 // 16-byte reads at one.
+// Memory-bound: what counts is how many regions a CU has in flight.  bf16 is held as it is read, which with 16 KiB of LDS lets
+// eight workgroups share a CU: 16384 x 4096 bf16 39.4 us by tiles, 45.8 transposed (5.1 and 4.4 TB/s; widened at once, with six
+// workgroups, 50.1 and 55.4); f32 64.0 and 70.2 us (5.2 and 4.8 TB/s).
 template <typename SRC, bool TILES, bool TRANS>
 __global__ __launch_bounds__(256) void quantize_region_kernel(QuantArgs p) {
   static_assert(TILES || TRANS, "rows are quantize_rows_kernel's");
@@ -122,14 +137,15 @@ __global__ __launch_bounds__(256) void quantize_region_kernel(QuantArgs p) {
   const int regions_c = (p.cols + 127) / 128;
   const int br = blockIdx.x / regions_c, bc = blockIdx.x % regions_c;
   const int col = bc * 128 + c16 * 8;
-  __shared__ unsigned red[TILES ? 1 : 16][128];
+  // the maxima, and in their place the transposed image when they have been read
   __shared__ __attribute__((aligned(16))) unsigned turned[TRANS ? 128 * 32 : 4];
+  unsigned(*const red)[128] = (unsigned(*)[128])turned;
 
-  float x[2][4][8];
+  Eight<SRC> x[2][4];
 #pragma unroll
   for (int h = 0; h < 2; h++)
 #pragma unroll
-    for (int r = 0; r < 4; r++) load8<SRC>(p, br * 128 + rg * 4 + r + 64 * h, col, x[h][r]);
+    for (int r = 0; r < 4; r++) x[h][r] = load8<SRC>(p, br * 128 + rg * 4 + r + 64 * h, col);
 
   float inv[TILES ? 1 : 8];
   if constexpr (!TILES) {
@@ -155,6 +171,7 @@ __global__ __launch_bounds__(256) void quantize_region_kernel(QuantArgs p) {
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 8; j++) inv[j] = __builtin_bit_cast(float, red[0][c16 * 8 + j]);
+    __syncthreads();
   } else {
     unsigned m = 0;
 #pragma unroll
@@ -163,14 +180,22 @@ __global__ __launch_bounds__(256) void quantize_region_kernel(QuantArgs p) {
       for (int r = 0; r < 4; r++) m = max(m, magnitude8(x[h][r]));
 #pragma unroll
     for (int off = 32; off; off >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, off, 64));
-    if ((t & 63) == 0) red[0][t >> 6] = m;
+    if ((t & 63) == 0) turned[t >> 6] = m;
     __syncthreads();
-    m = max(max(red[0][0], red[0][1]), max(red[0][2], red[0][3]));
+    m = max(max(turned[0], turned[1]), max(turned[2], turned[3]));
+    if constexpr (TRANS) __syncthreads();
     float scale;
     scale_of(m, &scale, &inv[0]);
     if (t == 0) p.scales[TRANS ? (int64_t)bc * p.ld_scales + br : (int64_t)br * p.ld_scales + bc] = scale;
   }
 
+  if constexpr (sizeof(SRC) == 2) {
+    // widened once more below: kept as f32 from here on they would be 64 registers in place of 32
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) asm volatile("" : "+v"(x[h][r].v));
+  }
   if constexpr (!TRANS) {
     const int last16 = (p.cols + 15) & ~15;
 #pragma unroll
@@ -178,7 +203,7 @@ __global__ __launch_bounds__(256) void quantize_region_kernel(QuantArgs p) {
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const int row = br * 128 + rg * 4 + r + 64 * h;
-        const float(&v)[8] = x[h][r];
+        const Eight<SRC>& v = x[h][r];
         if (row < p.rows && col < last16)
           store(p, p.dst + (int64_t)row * p.ld_dst + col, u32x2{e4m3x4(v[0] * inv[0], v[1] * inv[0], v[2] * inv[0], v[3] * inv[0]),
                                                                 e4m3x4(v[4] * inv[0], v[5] * inv[0], v[6] * inv[0], v[7] * inv[0])});
@@ -246,7 +271,6 @@ int gmd_block_quantize_launch(const gmd_block_quantize_t* q, void* hip_stream) {
   if (p.ld_src < q->cols) return refuse("a source row stride shorter than a row");
   if (p.ld_dst < c16 || p.ld_dst % 16) return refuse("a result row stride that is not a multiple of 16 or shorter than a row rounded up to 16");
   if (p.ld_scales < (q->blocks == GMD_BLOCK_ROWS ? r : kb)) return refuse("a stride of scales shorter than what it spans");
-  p.vec = (((uintptr_t)p.src | (uintptr_t)(p.ld_src * elem)) & 15) == 0;
   // A result that the caches would keep for the product that reads it is stored through them; a larger one is not (16384 x 7168:
   // 56.3 against 68.2 us).  32 MiB: the L2s of the eight XCDs together.
   p.stream = r * c16 > (32 << 20);
