@@ -195,8 +195,10 @@ GMD_API int gmd_mx_pack_scales(const void* scales_row_major, void* packed, int r
 
 /* ------------------------------------- fp8 in blocks of 128, and GEMMs by expert -- */
 /* e4m3 with one f32 scale per block of 128: what a mixture-of-experts job feeds its products.  All launches below work on
- * caller memory of the current device, are asynchronous in `hip_stream`, need no workspace, read nothing back to the host
- * and can be captured into a graph.  A stride of 0 means packed.  A size of zero is no error. */
+ * caller memory of the stream's device (operands on another one are refused), are asynchronous in `hip_stream`, need no
+ * workspace, read nothing back to the host and can be captured into a graph.  A stride of 0 means packed; results do not
+ * overlap operands.  A size of zero is no error: an empty result is left alone, a sum over nothing is zero.  Sizes up to
+ * 2^31 - 1024, 2^20 experts. */
 typedef enum {
   GMD_BLOCK_ROWS = 0,  /* 128 consecutive elements of a row share a scale; scales[kb * ld_scales + row] */
   GMD_BLOCK_TILES = 1  /* 128 x 128 elements do;                          scales[(row / 128) * ld_scales + kb] */
@@ -207,7 +209,7 @@ typedef enum {
  * rounded to nearest, ties to even.  The result's rows are filled up to the next multiple of 16 with zeros (ld_dst is a
  * multiple of 16, dst 16-byte aligned); blocks at the end of a row or at the bottom may be partial.  A block holding an
  * infinity or a NaN gets an infinite or NaN scale, so that every product that reads it is NaN.
- * Any rows, cols and ld_src >= cols; src rows that are 16-byte aligned are read in 16-byte pieces. */
+ * Any rows, cols and ld_src >= cols, src aligned to its elements. */
 typedef struct {
   const void* src;
   void* dst;

@@ -19,8 +19,8 @@ extern "C" {
 
 int gmd_gemm_block_launch(const gmd_gemm_block_t* g, void* hip_stream) {
   using namespace gmd::tiles;
-  if (!g || g->m < 0 || g->n < 0 || g->k < 0) {
-    gmd::set_error("block GEMM: negative sizes");
+  if (!g || g->m < 0 || g->n < 0 || g->k < 0 || std::max({g->m, g->n, g->k}) > kMaxSize) {
+    gmd::set_error("block GEMM: negative sizes, or sizes over 2^31 - 1024");
     return GMD_ERR_BADPARAM;
   }
   if (g->n % 8 || g->k % 16) {
@@ -40,14 +40,14 @@ int gmd_gemm_block_launch(const gmd_gemm_block_t* g, void* hip_stream) {
   p.ld_sa = g->ld_scale_a ? g->ld_scale_a : g->m;
   p.ld_sb = g->ld_scale_b ? g->ld_scale_b : g->b_blocks == GMD_BLOCK_TILES ? kb : g->n;
   p.a = (const char*)g->a, p.b = (const char*)g->b, p.c = g->c, p.sa = g->scale_a, p.sb = g->scale_b;
-  const int out_bytes = g->out_dtype == GMD_DT_BF16 ? 2 : 4;
-  const char* bad = bad_operand(g->c, p.ldc * out_bytes, (int64_t)g->n * out_bytes);
+  const char* bad = bad_operand(g->c, p.ldc, g->n, g->out_dtype == GMD_DT_BF16 ? 2 : 4);
   if (!bad && g->k > 0) {
-    bad = bad_operand(g->a, p.lda, g->k);
-    if (!bad) bad = bad_operand(g->b, p.ldb, g->k);
+    bad = bad_operand(g->a, p.lda, g->k, 1);
+    if (!bad) bad = bad_operand(g->b, p.ldb, g->k, 1);
     if (!bad && (!p.sa || !p.sb || (((uintptr_t)p.sa | (uintptr_t)p.sb) & 3))) bad = "null or misaligned scales";
     if (!bad && (p.ld_sa < g->m || p.ld_sb > 1 << 28 || p.ld_sb < (g->b_blocks == GMD_BLOCK_TILES ? kb : g->n))) bad = "a stride of scales shorter than what it spans, or over 2^28";
   }
+  if (!bad) bad = gmd::elsewhere((hipStream_t)hip_stream, {g->a, g->b, g->c});
   if (bad) {
     gmd::set_error("block GEMM: %s", bad);
     return GMD_ERR_BADPARAM;

@@ -260,7 +260,8 @@ int gmd_block_quantize_launch(const gmd_block_quantize_t* q, void* hip_stream) {
     gmd::set_error("block quantise: %s", why);
     return GMD_ERR_BADPARAM;
   };
-  if (!q || q->rows < 0 || q->cols < 0) return refuse("negative sizes");
+  constexpr int kMaxSize = 0x7fffffff - 1023;  // rounded up to a region it still fits 31 bits
+  if (!q || q->rows < 0 || q->cols < 0 || q->rows > kMaxSize || q->cols > kMaxSize) return refuse("negative sizes, or sizes over 2^31 - 1024");
   if (q->src_dtype != GMD_DT_BF16 && q->src_dtype != GMD_DT_F32) return refuse("the source is bf16 or f32");
   if (q->blocks != GMD_BLOCK_ROWS && q->blocks != GMD_BLOCK_TILES) return refuse("blocks are rows or tiles");
   if (q->rows == 0 || q->cols == 0) return GMD_OK;
@@ -277,6 +278,7 @@ int gmd_block_quantize_launch(const gmd_block_quantize_t* q, void* hip_stream) {
   if (p.ld_src < q->cols) return refuse("a source row stride shorter than a row");
   if (p.ld_dst < c16 || p.ld_dst % 16) return refuse("a result row stride that is not a multiple of 16 or shorter than a row rounded up to 16");
   if (p.ld_scales < (q->blocks == GMD_BLOCK_ROWS ? r : kb)) return refuse("a stride of scales shorter than what it spans");
+  if (const char* bad = gmd::elsewhere((hipStream_t)hip_stream, {p.src, p.dst})) return refuse(bad);
   // A result that the caches would keep for the product that reads it is stored through them; a larger one is not (16384 x 7168:
   // 56.3 against 68.2 us).  32 MiB: the L2s of the eight XCDs together.
   p.stream = r * c16 > (32 << 20);

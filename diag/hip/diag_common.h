@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <string>
 #include <vector>
 
@@ -46,6 +47,23 @@ inline void span_plan(uint64_t n, uint64_t pass, unsigned max_grid, unsigned* gr
   uint64_t per = (passes + g - 1) / g;
   *span = per * pass;
   *grid = (unsigned)std::max<uint64_t>(1, (n + *span - 1) / *span);
+}
+
+// Why operands cannot be used on this stream, or null: memory of another GPU than the stream's would be read over the links
+// where peers are mapped and fault where they are not.  Host memory and what the runtime does not know are left to the caller.
+inline const char* elsewhere(hipStream_t stream, std::initializer_list<const void*> operands) {
+  int here = 0;
+  if ((stream ? hipStreamGetDevice(stream, &here) : hipGetDevice(&here)) != hipSuccess) {
+    (void)hipGetLastError();  // (the launch that follows reports what is wrong)
+    return nullptr;
+  }
+  for (const void* p : operands) {
+    hipPointerAttribute_t at;
+    if (!p) continue;
+    if (hipPointerGetAttributes(&at, p) != hipSuccess) (void)hipGetLastError();
+    else if (at.type == hipMemoryTypeDevice && at.device != here) return "an operand on another device than the stream's";
+  }
+  return nullptr;
 }
 
 struct DeviceBuffer {

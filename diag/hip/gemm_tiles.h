@@ -90,7 +90,7 @@ struct RowTiles {
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const int v = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += v;
+      if (lane >= off) upto = __builtin_elementwise_add_sat(upto, v);  // (offsets that descend can sum to more than 31 bits)
     }
   }
   __device__ __forceinline__ void init(const Args& p, int bm_, int bn_) {
@@ -102,8 +102,9 @@ struct RowTiles {
     total = 0;
     for (int g0 = 0; g0 < p.groups; g0 += 64) {
       scan(p, g0);
-      total += __builtin_amdgcn_readlane(upto, 63);
+      total = __builtin_elementwise_add_sat(total, __builtin_amdgcn_readlane(upto, 63));
     }
+    total = min(total, (p.m / bm + min(p.groups, p.m)) * tiles_n);  // as the host's grid; offsets that ascend stay under it
   }
   __device__ __forceinline__ bool find(const Args& p, int id, Tile* t) {
     if (id >= total) return false;
@@ -122,12 +123,12 @@ struct RowTiles {
       if (has) {
         const int l = __builtin_ctzll(has);  // the first expert whose tiles reach past this one
         const int glo = __builtin_amdgcn_readlane(lo, l), ghi = __builtin_amdgcn_readlane(hi, l);
-        const int tiles_m = (ghi - glo + bm - 1) / bm, first = __builtin_amdgcn_readlane(upto, l) - tiles_m * tiles_n;
+        const int tiles_m = (ghi - glo + bm - 1) / bm, first = l ? __builtin_amdgcn_readlane(upto, l - 1) : 0;
         tile_walk(in - first, tiles_m, tiles_n, &tm, &tn);
         t->group = g0 + l, t->m0 = glo + tm * bm, t->m_end = ghi, t->n0 = tn * bn;
         return true;
       }
-      before += __builtin_amdgcn_readlane(upto, 63);
+      before = __builtin_elementwise_add_sat(before, __builtin_amdgcn_readlane(upto, 63));
     }
     return false;
   }
@@ -363,16 +364,12 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   int64_t k_first = 0;
   int K = p.k;
   RowTiles tiles;
-  const int ids = WGRAD ? p.groups * (((p.m + BM - 1) / BM * ((p.n + BN - 1) / BN) + 7) / 8 * 8) : 0;
   if constexpr (!WGRAD) tiles.init(p, BM, BN);
   int id = blockIdx.x;
   auto locate = [&]() {
-    bool found = false;
-    if constexpr (WGRAD) {
-      for (; id < ids && !found; id += found ? 0 : gridDim.x) found = wgrad_tile(p, BM, BN, id, &t, &k_first, &K);
-    } else {
-      found = tiles.find(p, id, &t);
-    }
+    bool found;
+    if constexpr (WGRAD) found = wgrad_tile(p, BM, BN, id, &t, &k_first, &K);
+    else found = tiles.find(p, id, &t);
     // (uniform as they are; said so, the compiler keeps them, and the DMA's base addresses, in scalar registers across the loop)
     t.group = __builtin_amdgcn_readfirstlane(t.group), t.m0 = __builtin_amdgcn_readfirstlane(t.m0);
     t.m_end = __builtin_amdgcn_readfirstlane(t.m_end), t.n0 = __builtin_amdgcn_readfirstlane(t.n0);
@@ -820,8 +817,10 @@ inline int64_t grid_for(const Args& p, bool wgrad, int bm, int bn) {
   const int64_t tiles = (((int64_t)p.m + bm - 1) / bm) * (((int64_t)p.n + bn - 1) / bn);
   return p.groups * ((tiles + 7) / 8 * 8);  // wgrad_tile
 }
+// Sizes and grids up to here: rounded up to a tile, or a round of workgroups further, they still fit 31 bits.
+constexpr int kMaxSize = 0x7fffffff - 1023;
 inline int launched(const char* what, int64_t grid) {
-  if (grid <= 0 || grid > 0x7fffffff) {
+  if (grid <= 0 || grid > kMaxSize) {
     set_error("%s: %lld workgroups do not fit into one launch", what, (long long)grid);
     return GMD_ERR_BADPARAM;
   }
@@ -878,7 +877,7 @@ int launch_few(const Args& p, hipStream_t st) {
 }
 template <int KIND, typename OUT>
 int launch_forward(const Args& p, hipStream_t st) {
-  const int rows = p.offsets ? (p.m + p.groups - 1) / p.groups : p.m;
+  const int rows = p.offsets ? (int)(((int64_t)p.m + p.groups - 1) / p.groups) : p.m;
   const int mb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   const int nb = grid_of(p, 16 * mb, 16) <= kCUs ? 1 : grid_of(p, 16 * mb, 32) <= kCUs ? 2 : grid_of(p, 16 * mb, 64) <= kCUs ? 4 : 0;
   if (mb == 1) {
@@ -909,13 +908,13 @@ int launch_forward(const Args& p, hipStream_t st) {
 // Block-scaled fp8, one product or one per expert (block_gemm.hip).
 int launch_fp8(const Args& p, int b_blocks, int out_dtype, hipStream_t st);
 // Shared refusals: null when the pointer, the row stride and the extent fit the kernels, else what is wrong.
-// row_bytes: what a row holds; the lane offsets inside a 256-row tile are 32 bits, hence the limit on ld_bytes.
-inline const char* bad_operand(const void* p, int64_t ld_bytes, int64_t row_bytes) {
+// ld and row in elements of `elem` bytes; the lane offsets inside a 256-row tile are 32 bits, hence the limit on the stride.
+inline const char* bad_operand(const void* p, int64_t ld, int64_t row, int elem) {
   if (!p) return "a null pointer";
   if ((uintptr_t)p & 15) return "a pointer that is not 16-byte aligned";
-  if (ld_bytes & 15) return "a row stride that is not a multiple of 16 bytes";
-  if (ld_bytes < row_bytes) return "a row stride shorter than a row";
-  if (ld_bytes > (8 << 20)) return "a row stride over 8 MiB";
+  if (ld < row) return "a row stride shorter than a row";
+  if (ld > (8 << 20) / elem) return "a row stride over 8 MiB";
+  if (ld * elem & 15) return "a row stride that is not a multiple of 16 bytes";
   return nullptr;
 }
 

@@ -14,7 +14,7 @@ int launch_bf16(int op, const Args& p, hipStream_t st) {
   if (op == GMD_GROUPED_FORWARD) return launch_forward<kBf16, OUT>(p, st);
   if (op == GMD_GROUPED_DGRAD) {
     // As in the forward, but always 64 columns a workgroup: a row of W is read in pieces of that many.
-    const int rows = (p.m + p.groups - 1) / p.groups;
+    const int rows = (int)(((int64_t)p.m + p.groups - 1) / p.groups);
     if (rows <= 16) return launch_few<kBf16, false, true, 1, 4, 8, 1, OUT>(p, st);
     if (rows <= 32) return launch_few<kBf16, false, true, 2, 4, 6, 1, OUT>(p, st);
     if (grid_of(p, 64, 64) <= 2 * kCUs) return launch_few<kBf16, false, true, 4, 4, 4, 1, OUT>(p, st);
@@ -22,7 +22,7 @@ int launch_bf16(int op, const Args& p, hipStream_t st) {
   }
   if (grid_for(p, true, 64, 64) <= 2 * kCUs) return launch_few<kBf16, true, true, 4, 4, 4, 1, OUT>(p, st);
   Args one = p;  // an expert's share of the rows is its contraction
-  one.offsets = nullptr, one.k = (p.k + p.groups - 1) / p.groups, one.m = p.m;
+  one.offsets = nullptr, one.k = (int)(((int64_t)p.k + p.groups - 1) / p.groups);
   const double steps = std::ceil(one.k / 64.0);
   return TileCost::large(p.groups * tiles_of(one, 256, 256), steps) < TileCost::small(p.groups * tiles_of(one, 128, 128), steps)
              ? launch_tile<kBf16, true, true, 256, 256, 2, 4, OUT>(p, st)
@@ -41,7 +41,8 @@ int gmd_grouped_gemm_launch(const gmd_grouped_gemm_t* g, void* hip_stream) {
     gmd::set_error("grouped GEMM: %s", why);
     return GMD_ERR_BADPARAM;
   };
-  if (!g || g->rows < 0 || g->n < 0 || g->k < 0 || g->groups < 0) return refuse("negative sizes");
+  if (!g || std::min({g->rows, g->n, g->k, g->groups}) < 0 || std::max({g->rows, g->n, g->k}) > kMaxSize || g->groups > 1 << 20)
+    return refuse("negative sizes, sizes over 2^31 - 1024, or more than 2^20 experts");
   if (g->op != GMD_GROUPED_FORWARD && g->op != GMD_GROUPED_DGRAD && g->op != GMD_GROUPED_WGRAD) return refuse("op is forward, dgrad or wgrad");
   if (g->dtype != GMD_DT_BF16 && g->dtype != GMD_DT_FP8) return refuse("operands are bf16 or fp8");
   if (g->out_dtype != GMD_DT_BF16 && g->out_dtype != GMD_DT_F32) return refuse("the result is bf16 or f32");
@@ -49,18 +50,17 @@ int gmd_grouped_gemm_launch(const gmd_grouped_gemm_t* g, void* hip_stream) {
   if (fp8 && g->op != GMD_GROUPED_FORWARD)
     return refuse("fp8 runs forward only: the input gradient is a forward with transposed weights, the weight gradient is taken in bf16");
   if (g->n % 8 || g->k % (fp8 ? 16 : 8)) return refuse("N in multiples of 8, K in multiples of 8 (bf16) or 16 (fp8)");
-  if (g->n == 0 || g->groups == 0 || (g->k == 0 && g->op != GMD_GROUPED_FORWARD) || (g->rows == 0 && !wgrad)) return GMD_OK;
-  if (!g->offsets || ((uintptr_t)g->offsets & 3)) return refuse("null or misaligned offsets");
-
   const int elem = fp8 ? 1 : 2, out = g->out_dtype == GMD_DT_BF16 ? 2 : 4;
   const int64_t kb = ((int64_t)g->k + 127) / 128, nb = ((int64_t)g->n + 127) / 128;
   const int64_t a_cols = g->op == GMD_GROUPED_FORWARD ? g->k : g->n;
   const int64_t c_cols = g->op == GMD_GROUPED_FORWARD ? g->n : g->k;
+  if (c_cols == 0 || g->groups == 0 || (wgrad ? g->n : g->rows) == 0) return GMD_OK;  // an empty result
+  if (!g->offsets || ((uintptr_t)g->offsets & 3)) return refuse("null or misaligned offsets");
   const int64_t lda = g->lda ? g->lda : a_cols, ldb = g->ldb ? g->ldb : g->k, ldc = g->ldc ? g->ldc : c_cols;
   const int64_t stride_w = g->stride_w ? g->stride_w : (int64_t)g->n * (wgrad ? ldc : ldb);
-  const char* bad = bad_operand(g->c, ldc * out, c_cols * out);
-  if (!bad && a_cols > 0 && g->rows > 0) bad = bad_operand(g->a, lda * elem, a_cols * elem);
-  if (!bad && g->k > 0 && (!wgrad || g->rows > 0)) bad = bad_operand(g->b, ldb * elem, (int64_t)g->k * elem);
+  const char* bad = bad_operand(g->c, ldc, c_cols, out);
+  if (!bad && a_cols > 0 && g->rows > 0) bad = bad_operand(g->a, lda, a_cols, elem);
+  if (!bad && (wgrad ? g->rows > 0 : g->n > 0 && g->k > 0)) bad = bad_operand(g->b, ldb, g->k, elem);
   if (!bad && (stride_w * (wgrad ? out : elem) % 16 || stride_w < (int64_t)(g->n - 1) * (wgrad ? ldc : ldb) + g->k))
     bad = "an expert stride that is not a multiple of 16 bytes or shorter than an expert";
   Args p;
@@ -80,6 +80,7 @@ int gmd_grouped_gemm_launch(const gmd_grouped_gemm_t* g, void* hip_stream) {
     if (!p.sa || !p.sb || (((uintptr_t)p.sa | (uintptr_t)p.sb) & 3)) bad = "null or misaligned scales";
     else if (p.ld_sa < g->rows || p.ld_sb > 1 << 28 || p.ld_sb < kb || p.stride_sb < (nb - 1) * p.ld_sb + kb) bad = "a stride of scales shorter than what it spans, or over 2^28";
   }
+  if (!bad) bad = gmd::elsewhere((hipStream_t)hip_stream, {g->a, g->b, g->c});
   if (bad) return refuse(bad);
   if (fp8) return launch_fp8(p, GMD_BLOCK_TILES, g->out_dtype, (hipStream_t)hip_stream);
   return g->out_dtype == GMD_DT_BF16 ? launch_bf16<__bf16>(g->op, p, (hipStream_t)hip_stream)

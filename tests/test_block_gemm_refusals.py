@@ -43,6 +43,8 @@ def test_quantize_refusals(diag):
     refused(diag, "stride of scales", f, P, Q, R, 300, 200, ld_scales=299)
     refused(diag, "stride of scales", f, P, Q, R, 300, 200, blocks="tiles", ld_scales=1)
     refused(diag, "stride of scales", f, P, Q, R, 300, 200, blocks="tiles", transpose=True, ld_scales=2)
+    refused(diag, "over 2.31", f, P, Q, R, 0x7fffffff, 8)
+    refused(diag, "over 2.31", f, P, Q, R, 8, 0x7fffffff - 1022)
     refused(diag, "gmd_block_quantize_launch", f, P, Q, R, 1 << 31, 8)          # does not fit its field
     with pytest.raises(KeyError):
         f(P, Q, R, 8, 8, blocks="columns")
@@ -53,6 +55,8 @@ def test_quantize_refusals(diag):
 def test_gemm_block_refusals(diag):
     f = diag.gemm_block_launch
     refused(diag, "negative", f, P, R, Q, R, S, -1, 8, 16)
+    refused(diag, "over 2.31", f, P, R, Q, R, S, 0x7fffffff, 8, 16)
+    refused(diag, "over 2.31", f, P, R, Q, R, S, 8, 8, 0x7ffffff0)
     refused(diag, "multiples of 8", f, P, R, Q, R, S, 8, 12, 16)
     refused(diag, "multiples of 16", f, P, R, Q, R, S, 8, 8, 24)
     refused(diag, "bf16 or f32", f, P, R, Q, R, S, 8, 8, 16, out="fp8")
@@ -68,6 +72,7 @@ def test_gemm_block_refusals(diag):
     refused(diag, "shorter than a row", f, P, R, Q, R, S, 8, 32, 48, ldc=24)
     refused(diag, "shorter than a row", f, P, R, Q, R, S, 8, 32, 48, ldc=-32)
     refused(diag, "over 8 MiB", f, P, R, Q, R, S, 8, 8, 16, lda=(8 << 20) + 16)
+    refused(diag, "over 8 MiB", f, P, R, Q, R, S, 8, 8, 16, ldc=(1 << 62) + 1024, out="f32")  # must not wrap to a small one
     refused(diag, "stride of scales", f, P, R, Q, R, S, 8, 8, 16, ld_scale_a=7)
     refused(diag, "stride of scales", f, P, R, Q, R, S, 8, 16, 16, b_blocks="rows", ld_scale_b=8)
     refused(diag, "stride of scales", f, P, R, Q, R, S, 8, 16, 400, ld_scale_b=3)
@@ -80,6 +85,8 @@ def test_grouped_refusals(diag):
     size = (4, 100, 64, 64)  # groups, rows, n, k
     refused(diag, "negative", f, "forward", "bf16", P, Q, S, R, 4, -1, 64, 64)
     refused(diag, "negative", f, "forward", "bf16", P, Q, S, R, -4, 1, 64, 64)
+    refused(diag, "over 2.31", f, "forward", "bf16", P, Q, S, R, 4, 0x7fffffff, 64, 64)
+    refused(diag, "experts", f, "wgrad", "bf16", P, Q, S, R, (1 << 20) + 1, 8, 64, 64)
     refused(diag, "bf16 or fp8", f, "forward", "f32", P, Q, S, R, *size)
     refused(diag, "result", f, "forward", "bf16", P, Q, S, R, *size, out="mxfp8")
     refused(diag, "forward only", f, "dgrad", "fp8", P, Q, S, R, *size, scale_a=P, scale_b=P)
@@ -108,6 +115,8 @@ def test_grouped_refusals(diag):
     f("forward", "bf16", None, None, None, None, 4, 0, 64, 64)
     f("forward", "bf16", None, None, None, None, 0, 100, 64, 64)
     f("wgrad", "bf16", None, None, None, None, 4, 100, 0, 64)
+    f("dgrad", "bf16", None, None, None, None, 4, 100, 64, 0)
+    refused(diag, "null", f, "dgrad", "bf16", None, None, None, R, 4, 100, 0, 64)  # a sum over nothing is still written
 
 
 def test_packed_structs_match_the_header(diag, tmp_path):

@@ -210,6 +210,26 @@ def test_gemm_block_matches_64_bits(diag, dev, shape, b_blocks, out):
     assert_product(c, av @ bv.t(), av.abs() @ bv.abs().t(), k, k // 128 + 1)
 
 
+# more tiles of 256 x 256 than CUs: workgroups walk several, one's stores in flight under the next one's first steps
+@pytest.mark.parametrize("b_blocks", ["tiles", "rows"])
+@pytest.mark.parametrize("shape", [(5000, 5208, 16), (5000, 5208, 128), (5008, 5200, 272), (4992, 5200, 656), (5000, 5208, 1040)])
+def test_gemm_block_walks_many_large_tiles(diag, dev, shape, b_blocks):
+    m, n, k = shape
+    g = _gen(dev, m * 7 + n * 3 + k)
+    a, sa, av = make_blocks(m, k, "rows", dev, g)
+    b, sb, bv = make_blocks(n, k, b_blocks, dev, g)
+    ref, mag = av @ bv.t(), av.abs() @ bv.abs().t()
+    first = None
+    for _ in range(3):
+        raw, c = guarded(m, n, torch.bfloat16, dev)
+        diag.gemm_block_launch(a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(), c.data_ptr(), m, n, k, b_blocks=b_blocks, stream=_stream())
+        torch.cuda.synchronize()
+        assert guards_intact(raw)
+        assert_product(c, ref, mag, k, k // 128 + 1)
+        first = c.clone() if first is None else first
+        assert torch.equal(first.view(torch.int16), c.view(torch.int16))
+
+
 @pytest.mark.parametrize("b_blocks", ["tiles", "rows"])
 @pytest.mark.parametrize("m", [1, 40, 150, 1500])
 def test_gemm_block_strides_and_columns_left_alone(diag, dev, m, b_blocks):
@@ -400,6 +420,22 @@ def test_grouped_matches_64_bits(diag, dev, op, dtype, rows, groups, n, k, kind)
     run_grouped(diag, dev, op, dtype, rows, groups, n, k, split(rows, groups, rows, kind))
 
 
+@pytest.mark.parametrize("kind", ["even", "random", "one", "sparse"])
+@pytest.mark.parametrize("depth", [16, 64, 144, 400, 1040])
+@pytest.mark.parametrize("op,dtype,out", [("forward", "bf16", "bf16"), ("forward", "bf16", "f32"), ("forward", "fp8", "bf16"), ("dgrad", "bf16", "bf16"),
+                                          ("dgrad", "bf16", "f32")])
+def test_grouped_walks_many_large_tiles(diag, dev, op, dtype, out, depth, kind):
+    n, k = (4360, depth) if op == "forward" else (depth, 4360)
+    run_grouped(diag, dev, op, dtype, 6000, 3, n, k, split(6000, 3, depth, kind), out=out)
+
+
+@pytest.mark.parametrize("kind", ["even", "random", "one", "sparse"])
+@pytest.mark.parametrize("rows", [1, 40, 500, 3000])
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_grouped_weight_gradient_in_large_tiles(diag, dev, rows, out, kind):
+    run_grouped(diag, dev, "wgrad", "bf16", rows, 3, 1304, 2600, split(rows, 3, rows, kind), out=out)
+
+
 @pytest.mark.parametrize("op,dtype", OPS)
 @pytest.mark.parametrize("rows,groups", [(40, 9), (600, 5), (6000, 4)])
 def test_grouped_strides_f32_results_and_rows_of_no_expert(diag, dev, op, dtype, rows, groups):
@@ -432,6 +468,32 @@ def test_grouped_offsets_out_of_range_touch_nothing_outside(diag, dev, op, dtype
                                  scale_b=sb.data_ptr(), stream=_stream())
         torch.cuda.synchronize()
         assert guards_intact(raw) and bool(c.isfinite().all())
+
+
+@pytest.mark.parametrize("op,dtype,n,k", [("forward", "bf16", 1032, 144), ("forward", "fp8", 1032, 144), ("dgrad", "bf16", 144, 1032)])
+@pytest.mark.parametrize("groups", [40, 150])
+def test_grouped_offsets_up_and_down_over_many_tiles(diag, dev, op, dtype, n, k, groups):
+    """Every other expert owns all rows: more tiles than a launch has."""
+    rows = 6000
+    g = _gen(dev, 4)
+    kind = torch.bfloat16 if dtype == "bf16" else torch.float8_e4m3fn
+    a = torch.randn(rows, k if op == "forward" else n, device=dev, generator=g).to(kind)
+    b = torch.randn(groups, n, k, device=dev, generator=g).to(kind)
+    sa, sb = torch.ones(_up(k, 128) // 128, rows, device=dev), torch.ones(groups, _up(n, 128) // 128, _up(k, 128) // 128, device=dev)
+    raw, c = guarded(rows, n if op == "forward" else k, torch.bfloat16, dev)
+    offsets = torch.tensor([0, rows] * groups, dtype=torch.int32, device=dev)
+    diag.grouped_gemm_launch(op, dtype, a.data_ptr(), b.data_ptr(), c.data_ptr(), offsets.data_ptr(), groups, rows, n, k, scale_a=sa.data_ptr(),
+                             scale_b=sb.data_ptr(), stream=_stream())
+    torch.cuda.synchronize()
+    assert guards_intact(raw) and bool(c.isfinite().all())
+
+
+def test_grouped_input_gradient_of_no_columns_is_zero(diag, dev):
+    c = torch.full((70, 64), 7.0, dtype=torch.bfloat16, device=dev)
+    offsets = torch.tensor([3, 30, 30, 66], dtype=torch.int32, device=dev)
+    diag.grouped_gemm_launch("dgrad", "bf16", 0, 0, c.data_ptr(), offsets.data_ptr(), 3, 70, 0, 64, stream=_stream())
+    torch.cuda.synchronize()
+    assert bool((c[3:66] == 0).all()) and bool((c[:3] == 7.0).all()) and bool((c[66:] == 7.0).all())
 
 
 def test_grouped_empty_sizes(diag, dev):
