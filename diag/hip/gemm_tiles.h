@@ -583,6 +583,21 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
       read_scales(kt + 1);
     }
   };
+  // A wave whose part of the tile has no rows or columns of C keeps its share of the DMAs and the synchronisations and leaves the
+  // matrix pipe to the wave beside it.
+  auto idle_steps = [&]() {
+    if (steps > 1) sync(std::integral_constant<int, kFirst + 2 * kSecond>(), after_stores);
+    else sync(none);
+    for (int kt = 0; kt < steps; kt++) {
+      const bool more = kt + 1 < steps, more2 = kt + 2 < steps;
+      if (more) sync(step_behind, after_stores && kt <= 1);
+      else sync(none);
+      if (more2) fetch_edge(kt + 2, 0, kFirst);
+      if (more2) sync(step_behind, after_stores && kt == 0);
+      else sync(none);
+      if (more2) fetch_edge(kt + 2, kFirst, kFirst + kSecond);
+    }
+  };
   // Epilogue: kStripRows rows of a wave's tile at a time through a strip of LDS of its own, so that neighbouring lanes store
   // neighbouring columns of one row.
   constexpr int kCols16 = 16 / (int)sizeof(OUT);  // columns of a 16-byte store
@@ -636,12 +651,14 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
     for (int i = 0; i < MB; i++)
 #pragma unroll
       for (int j = 0; j < NB; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (steps > 0) first_fragments();
-    int kt = 0;
-    for (; kt + 2 < whole; kt++) step(kt, std::true_type());
-    for (; kt < steps; kt++) step(kt, std::false_type());
-    if constexpr (KIND == kFp8Tiles) {
-      if (steps > 0) {
+    if (t.m0 + wm * WTM >= t.m_end || t.n0 + wn * WTN >= p.n) {
+      if (steps > 0) idle_steps();
+    } else if (steps > 0) {
+      first_fragments();
+      int kt = 0;
+      for (; kt + 2 < whole; kt++) step(kt, std::true_type());
+      for (; kt < steps; kt++) step(kt, std::false_type());
+      if constexpr (KIND == kFp8Tiles) {
         add(kProducts - 2);
         add(kProducts - 1);
       }
@@ -651,7 +668,9 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
     const Tile o = t;
     bool next = false;
     if constexpr (MANY) {
-      id += gridDim.x;
+      // a round of ids on, and one place along this XCD's part of it: rows of tiles that an expert's end leaves part empty come at a
+      // fixed distance, and would all fall to the same workgroups
+      id = (id & ~(kCUs - 1)) + kCUs + ((id + 8) & (kCUs - 1));
       next = locate();
       if (next) {
         prepare();
