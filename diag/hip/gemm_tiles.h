@@ -343,33 +343,34 @@ struct Operand<2> {
 // Block-scaled fp8: the matrix instruction sums one block of 128 k from zero and its result is added with one FMA per
 // element, acc += (sa * sb) * block.  With rows dealt to lanes (Stage's DEAL) a lane's scales of A are MB consecutive floats
 // per K-step, and B's tile scale is one scalar per wave.
-template <int KIND, bool TA, bool TB, bool WGRAD, int BM, int BN, int WM, int WN, bool MANY, typename OUT>
-__global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
+template <int KIND, int BM, int BN, int WM, int WN, bool MANY, typename OUT>
+struct TileLds {  // two buffers of operands and scales; MANY: behind them the epilogue's strips, which else take their place
+  static constexpr bool kNarrow = sizeof(OUT) == 2;
+  static constexpr int kOperands = (BM + BN) * kStepBytes, kScales = KIND != kBf16 ? WM * WN * 256 : 0;
+  static constexpr int kStripRows = kNarrow ? 16 : 8, kStrip = BN / WN * (int)sizeof(OUT) + 16, kStrips = WM * WN * kStripRows * kStrip;
+  static_assert(kStrips <= 2 * kOperands, "the epilogue's strips fit into the operand buffers");
+  static constexpr int kBytes = 2 * (kOperands + kScales) + (MANY ? kStrips : 0);
+};
+// Computes the tiles that next(&tile, &k_first, &K) names until it returns false; without MANY one.
+template <int KIND, bool TA, bool TB, bool WGRAD, int BM, int BN, int WM, int WN, bool MANY, typename OUT, typename NEXT>
+__device__ __forceinline__ void compute_tiles(const Args& p, char* const smem, NEXT next_tile) {
   constexpr int kWaves = WM * WN, WTM = BM / WM, WTN = BN / WN, MB = WTM / 16, NB = WTN / 16;
   constexpr bool kFp8 = KIND != kBf16, kNarrow = sizeof(OUT) == 2;
   constexpr int kElem = kFp8 ? 1 : 2, kStepK = kStepBytes / kElem;
   static_assert(!kFp8 || (!TA && !TB && WTN <= 128), "block-scaled fp8: k contiguous, a wave's columns inside one tile of scales");
-  constexpr int kABytes = BM * kStepBytes, kBufBytes = (BM + BN) * kStepBytes;
-  constexpr int kStripRows = kNarrow ? 16 : 8, kStrip = WTN * (int)sizeof(OUT) + 16, kStripBytes = kStripRows * kStrip;  // epilogue, per wave
-  static_assert(kWaves * kStripBytes <= 2 * kBufBytes, "the epilogue's strips fit into the operand buffers");
-  constexpr int kScaleBytes = kFp8 ? kWaves * 256 : 0;
+  typedef TileLds<KIND, BM, BN, WM, WN, MANY, OUT> Lds;
+  constexpr int kABytes = BM * kStepBytes, kBufBytes = Lds::kOperands, kScaleBytes = Lds::kScales;
+  constexpr int kStripRows = Lds::kStripRows, kStrip = Lds::kStrip, kStripBytes = kStripRows * kStrip;
   static_assert(!kFp8 || BM / 64 + (KIND == kFp8Rows ? BN / 64 : 1) <= kWaves, "one DMA of scales per wave and step");
-  __shared__ __attribute__((aligned(16))) char smem[2 * (kBufBytes + kScaleBytes) + (MANY ? kWaves * kStripBytes : 0)];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
-  // The tile at hand; MANY: ids blockIdx.x, blockIdx.x + gridDim.x, ...
-  Tile t{0, 0, 0, 0};
+  Tile t{0, 0, 0, 0};  // the tile at hand
   int64_t k_first = 0;
   int K = p.k;
-  RowTiles tiles;
-  if constexpr (!WGRAD) tiles.init(p, BM, BN);
-  int id = blockIdx.x;
   auto locate = [&]() {
-    bool found;
-    if constexpr (WGRAD) found = wgrad_tile(p, BM, BN, id, &t, &k_first, &K);
-    else found = tiles.find(p, id, &t);
+    const bool found = next_tile(&t, &k_first, &K);
     // (uniform as they are; said so, the compiler keeps them, and the DMA's base addresses, in scalar registers across the loop)
     t.group = __builtin_amdgcn_readfirstlane(t.group), t.m0 = __builtin_amdgcn_readfirstlane(t.m0);
     t.m_end = __builtin_amdgcn_readfirstlane(t.m_end), t.n0 = __builtin_amdgcn_readfirstlane(t.n0);
@@ -668,9 +669,6 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
     const Tile o = t;
     bool next = false;
     if constexpr (MANY) {
-      // a round of ids on, and one place along this XCD's part of it: rows of tiles that an expert's end leaves part empty come at a
-      // fixed distance, and would all fall to the same workgroups
-      id = (id & ~(kCUs - 1)) + kCUs + ((id + 8) & (kCUs - 1));
       next = locate();
       if (next) {
         prepare();
@@ -684,6 +682,48 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
     else store_tile(o, std::false_type());
     if (!next) break;
     after_stores = full;
+  }
+}
+
+// MANY: kCUs workgroups walk the tiles, one of 256 x 256 a CU, ids blockIdx.x, blockIdx.x + kCUs, ...  What is left for a last
+// round of up to half the CUs is computed in quarters of those tiles, by twice or four times as many CUs.
+template <int KIND, bool TA, bool TB, bool WGRAD, int BM, int BN, int WM, int WN, bool MANY, typename OUT>
+__global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
+  typedef TileLds<KIND, BM, BN, WM, WN, MANY, OUT> Lds;
+  __shared__ __attribute__((aligned(16))) char smem[Lds::kBytes];
+  if constexpr (WGRAD) {
+    compute_tiles<KIND, TA, TB, WGRAD, BM, BN, WM, WN, false, OUT>(
+        p, smem, [&](Tile* t, int64_t* k_first, int* K) { return wgrad_tile(p, BM, BN, blockIdx.x, t, k_first, K); });
+  } else if constexpr (!MANY) {
+    compute_tiles<KIND, TA, TB, WGRAD, BM, BN, WM, WN, false, OUT>(p, smem, [&](Tile* t, int64_t*, int*) {
+      RowTiles tiles;
+      tiles.init(p, BM, BN);
+      return tiles.find(p, blockIdx.x, t);
+    });
+  } else {
+    RowTiles tiles;
+    tiles.init(p, BM, BN);
+    const int rest = tiles.total % kCUs, quartered = rest <= kCUs / 2 ? rest : 0, whole = tiles.total - quartered;
+    int id = blockIdx.x;
+    compute_tiles<KIND, TA, TB, WGRAD, BM, BN, WM, WN, true, OUT>(p, smem, [&](Tile* t, int64_t*, int*) {
+      if (id >= whole) return false;
+      const bool found = tiles.find(p, id, t);
+      // a round of ids on, and one place along this XCD's part of it: rows of tiles that an expert's end leaves part empty come at a
+      // fixed distance, and would all fall to the same workgroups
+      id = (id & ~(kCUs - 1)) + kCUs + ((id + 8) & (kCUs - 1));
+      return found;
+    });
+    typedef TileLds<KIND, BM / 2, BN / 2, 4, 2, false, OUT> Quarter;
+    static_assert(WM * WN == 8 && Quarter::kBytes <= Lds::kBytes, "the same waves and LDS");
+    for (int q = blockIdx.x; q < (quartered + 7) / 8 * 32; q += kCUs) {  // eight tiles at a time, so that an XCD has a tile's quarters
+      const int of = whole + q / 32 * 8 + q % 8, part = q / 8 % 4;
+      __syncthreads();  // the LDS of what came before
+      compute_tiles<KIND, TA, TB, WGRAD, BM / 2, BN / 2, 4, 2, false, OUT>(p, smem, [&](Tile* t, int64_t*, int*) {
+        if (!tiles.find(p, of, t)) return false;
+        t->m0 += part / 2 * (BM / 2), t->n0 += part % 2 * (BN / 2);
+        return t->m0 < t->m_end && t->n0 < p.n;
+      });
+    }
   }
 }
 
@@ -863,6 +903,10 @@ struct TileCost {
     return full * (1.2 * steps + 4) + (rest > 256 ? 1.2 * steps + 4 : rest > 0 ? 0.6 * steps + 4 : 0);
   }
   static double large(double tiles, double steps) { return std::ceil(tiles / 256) * (1.55 * steps + 8); }
+  static double walked(double tiles, double steps) {  // ... with a short last round in quarters (tile_kernel)
+    const double rest = tiles - 256 * std::floor(tiles / 256);
+    return large(tiles, steps) - (rest > 0 && rest <= 64 ? 0.95 * steps + 4 : rest > 0 && rest <= 128 ? 0.35 * steps : 0);
+  }
 };
 // Tiles that a launch really has: with experts about half a row of tiles each is cut off.
 inline double tiles_of(const Args& p, int bm, int bn) {
@@ -871,7 +915,7 @@ inline double tiles_of(const Args& p, int bm, int bn) {
 }
 inline bool large_tiles(const Args& p, int step_k) {
   const double steps = std::ceil(p.k / (double)step_k);
-  return TileCost::large(tiles_of(p, 256, 256), steps) < TileCost::small(tiles_of(p, 128, 128), steps);
+  return TileCost::walked(tiles_of(p, 256, 256), steps) < TileCost::small(tiles_of(p, 128, 128), steps);
 }
 
 template <int KIND, bool TA, bool TB, int BM, int BN, int WM, int WN, typename OUT>
@@ -881,7 +925,7 @@ int launch_tile(const Args& p, hipStream_t st) {
   // One large tile fits a CU: that many workgroups walk the tiles.  Not for the weight gradient, whose tiles cost what their experts
   // have of rows: dealt out one by one as CUs come free they take 302 us, in fixed turns 368 (16k rows, 16 experts of 4096 x 2048).
   constexpr bool kMany = BM * BN >= 256 * 256 && !TA;
-  if (kMany) grid = std::min<int64_t>(grid, kCUs);
+  if (kMany) grid = kCUs;
   tile_kernel<KIND, TA, TB, TA, BM, BN, WM, WN, kMany, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
   GMD_HIP(hipGetLastError());
   return GMD_OK;
