@@ -631,10 +631,12 @@ __device__ __forceinline__ void compute_tiles(const Args& p, char* const smem, N
           const int row = kFp8 ? (h * kStripRows + r0) * MB + i : i * 16 + h * kStripRows + r0;  // of the pass's first strip row
           char* const to = (char*)(base + row * p.ldc);
           const u32x4 v = *(const u32x4*)(strip + (r0 + strip_row) * kStrip + strip_col * (int)sizeof(OUT));
-          if constexpr (decltype(FULL)::value) {
-            // As asm, so that there are exactly kStores of them for the counted waits (and the wait state that a wide store's data
-            // needs).  Past the caches, which would not keep a result of that many tiles (8192^3 bf16 dgrad 764 -> 728 us).
+          // As asm, so that there are exactly kStores of them for the counted waits (and the wait state that a wide store's data
+          // needs).
+          if constexpr (decltype(FULL)::value == 2) {
             asm volatile("global_store_dwordx4 %0, %1, %2 nt\n\ts_nop 1" ::"v"(off), "v"(v), "s"(to) : "memory");
+          } else if constexpr (decltype(FULL)::value == 1) {
+            asm volatile("global_store_dwordx4 %0, %1, %2\n\ts_nop 1" ::"v"(off), "v"(v), "s"(to) : "memory");
           } else if (o.m0 + wm * WTM + row + strip_row * kApart < o.m_end && col_in) {
             *(u32x4*)(to + off) = v;
           }
@@ -645,6 +647,7 @@ __device__ __forceinline__ void compute_tiles(const Args& p, char* const smem, N
     }
   };
 
+  const bool lines = MANY && (((uintptr_t)p.c | (uintptr_t)(p.ldc * (int)sizeof(OUT))) & 127) == 0;
   prepare();
   begin();
   for (;;) {
@@ -678,8 +681,11 @@ __device__ __forceinline__ void compute_tiles(const Args& p, char* const smem, N
       __syncthreads();  // the strips lie in the operand buffers: every wave is done with them
     }
     const bool full = MANY && o.m0 + BM <= o.m_end && o.n0 + BN <= p.n;
-    if (full) store_tile(o, std::integral_constant<bool, MANY>());
-    else store_tile(o, std::false_type());
+    // Whole lines go past the caches, which would not keep a result of that many tiles (8192^3 bf16 dgrad 728 us, through them
+    // 764); rows that do not begin at a line share theirs with the next tile (5120 x 8184 x 352: 47.5 us through the caches, 58.0).
+    if (!full) store_tile(o, std::integral_constant<int, 0>());
+    else if (lines) store_tile(o, std::integral_constant<int, MANY ? 2 : 0>());
+    else store_tile(o, std::integral_constant<int, MANY ? 1 : 0>());
     if (!next) break;
     after_stores = full;
   }
@@ -963,9 +969,16 @@ int launch_forward(const Args& p, hipStream_t st) {
   if constexpr (KIND == kBf16 || sizeof(OUT) == 2)
     if (large_tiles(p, KIND == kBf16 ? 64 : 128)) return launch_tile<KIND, false, false, 256, 256, 2, 4, OUT>(p, st);
   // (widening costs a wave per fragment, not per product: four waves of 64 x 64 have fewer of them per product than eight of 32 x 64,
-  // 2048 x 7168 x 8192 276 against 326 us)
-  if constexpr (KIND != kBf16 && sizeof(OUT) == 4) return launch_tile<KIND, false, false, 128, 128, 2, 2, OUT>(p, st);
-  else return launch_tile<KIND, false, false, 128, 128, 4, 2, OUT>(p, st);
+  // 2048 x 7168 x 8192 276 against 326 us.  With one workgroup or none on a CU four waves are too few to hide their latencies, and
+  // either eight are better, 3584 x 1024 x 7168 by rows 75 against 96 us, or, where it has B's scales as scalars, the few-row kernel,
+  // by tiles 65 against 89)
+  if constexpr (KIND != kBf16 && sizeof(OUT) == 4) {
+    if (grid_of(p, 128, 128) > kCUs) return launch_tile<KIND, false, false, 128, 128, 2, 2, OUT>(p, st);
+    if constexpr (KIND == kFp8Tiles) return launch_few<KIND, false, false, 4, 4, 4, 1, OUT>(p, st);
+    else return launch_tile<KIND, false, false, 128, 128, 4, 2, OUT>(p, st);
+  } else {
+    return launch_tile<KIND, false, false, 128, 128, 4, 2, OUT>(p, st);
+  }
 }
 
 // Block-scaled fp8, one product or one per expert (block_gemm.hip).
