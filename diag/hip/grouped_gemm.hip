@@ -13,10 +13,14 @@ template <typename OUT>
 int launch_bf16(int op, const Args& p, hipStream_t st) {
   if (op == GMD_GROUPED_FORWARD) return launch_forward<kBf16, OUT>(p, st);
   if (op == GMD_GROUPED_DGRAD) {
-    // As in the forward, but always 64 columns a workgroup: a row of W is read in pieces of that many.
+    // As in the forward, but always 64 columns a workgroup: a row of W is read in pieces of that many.  Six waves leave room for two
+    // workgroups a CU (64 experts of 4096 x 2048 for 300 rows: 167 us, eight waves 176, four 191); with two blocks of rows and a
+    // K of up to 32 steps four are better, three workgroups of which fit (117 experts of 384 x 784 for 2398 rows 21 us, six 38;
+    // 64 experts of 2048 x 2048 for 1500 rows 116 and 125; but 8 experts of 4096 x 4096 for 200 rows 59 and 53).
     const int rows = (int)(((int64_t)p.m + p.groups - 1) / p.groups);
-    if (rows <= 16) return launch_few<kBf16, false, true, 1, 4, 8, 1, OUT>(p, st);
-    if (rows <= 32) return launch_few<kBf16, false, true, 2, 4, 6, 1, OUT>(p, st);
+    if (rows <= 16) return launch_few<kBf16, false, true, 1, 4, 6, 1, OUT>(p, st);
+    if (rows <= 32)
+      return p.k <= 32 * 64 ? launch_few<kBf16, false, true, 2, 4, 4, 1, OUT>(p, st) : launch_few<kBf16, false, true, 2, 4, 6, 1, OUT>(p, st);
     if (grid_of(p, 64, 64) <= 2 * kCUs) return launch_few<kBf16, false, true, 4, 4, 4, 1, OUT>(p, st);
     return large_tiles(p, 64) ? launch_tile<kBf16, false, true, 256, 256, 2, 4, OUT>(p, st) : launch_tile<kBf16, false, true, 128, 128, 4, 2, OUT>(p, st);
   }
