@@ -701,9 +701,21 @@ template <int KIND, bool TA, bool TB, bool WGRAD, int BM, int BN, int WM, int WN
 __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   typedef TileLds<KIND, BM, BN, WM, WN, MANY, OUT> Lds;
   __shared__ __attribute__((aligned(16))) char smem[Lds::kBytes];
+  // MANY: a round of ids on, and 17 of 32 places along this XCD's part of it: what comes at a fixed distance and costs more or less
+  // than the rest (rows of tiles that an expert's end leaves part empty, experts) would fall to the same workgroups (32 experts of
+  // 640 rows, 4096 x 7168 e4m3: 556 us; one place 580, none 645).
+  int id = blockIdx.x;
+  auto next_id = [&]() { return (id & ~(kCUs - 1)) + kCUs + ((id + 17 * 8) & (kCUs - 1)); };
   if constexpr (WGRAD) {
-    compute_tiles<KIND, TA, TB, WGRAD, BM, BN, WM, WN, false, OUT>(
-        p, smem, [&](Tile* t, int64_t* k_first, int* K) { return wgrad_tile(p, BM, BN, blockIdx.x, t, k_first, K); });
+    const int ids = p.groups * (((p.m + BM - 1) / BM * ((p.n + BN - 1) / BN) + 7) / 8 * 8);
+    compute_tiles<KIND, TA, TB, WGRAD, BM, BN, WM, WN, MANY, OUT>(p, smem, [&](Tile* t, int64_t* k_first, int* K) {
+      bool found = false;
+      while (!found && id < ids) {
+        found = wgrad_tile(p, BM, BN, id, t, k_first, K);
+        id = MANY ? next_id() : ids;
+      }
+      return found;
+    });
   } else if constexpr (!MANY) {
     compute_tiles<KIND, TA, TB, WGRAD, BM, BN, WM, WN, false, OUT>(p, smem, [&](Tile* t, int64_t*, int*) {
       RowTiles tiles;
@@ -714,13 +726,10 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
     RowTiles tiles;
     tiles.init(p, BM, BN);
     const int rest = tiles.total % kCUs, quartered = rest <= kCUs / 2 ? rest : 0, whole = tiles.total - quartered;
-    int id = blockIdx.x;
     compute_tiles<KIND, TA, TB, WGRAD, BM, BN, WM, WN, true, OUT>(p, smem, [&](Tile* t, int64_t*, int*) {
       if (id >= whole) return false;
       const bool found = tiles.find(p, id, t);
-      // a round of ids on, and one place along this XCD's part of it: rows of tiles that an expert's end leaves part empty come at a
-      // fixed distance, and would all fall to the same workgroups
-      id = (id & ~(kCUs - 1)) + kCUs + ((id + 8) & (kCUs - 1));
+      id = next_id();
       return found;
     });
     typedef TileLds<KIND, BM / 2, BN / 2, 4, 2, false, OUT> Quarter;
@@ -928,15 +937,13 @@ inline bool large_tiles(const Args& p, int step_k) {
   return TileCost::walked(tiles_of(p, 256, 256), steps) < TileCost::small(tiles_of(p, 128, 128), steps);
 }
 
-template <int KIND, bool TA, bool TB, int BM, int BN, int WM, int WN, typename OUT>
+template <int KIND, bool TA, bool TB, int BM, int BN, int WM, int WN, typename OUT, bool MANY = (BM * BN >= 256 * 256)>
 int launch_tile(const Args& p, hipStream_t st) {
   int64_t grid = grid_for(p, TA, BM, BN);
   if (int rc = launched("GEMM", grid)) return rc;
-  // One large tile fits a CU: that many workgroups walk the tiles (8192^3 e4m3, launched one by one: 455 us, 440).  Not for the weight gradient, whose tiles cost what their experts
-  // have of rows: dealt out one by one as CUs come free they take 302 us, in fixed turns 368 (16k rows, 16 experts of 4096 x 2048).
-  constexpr bool kMany = BM * BN >= 256 * 256 && !TA;
-  if (kMany) grid = kCUs;
-  tile_kernel<KIND, TA, TB, TA, BM, BN, WM, WN, kMany, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
+  // One large tile fits a CU: that many workgroups walk the tiles (8192^3 e4m3 440 us, launched one by one 455).
+  if (MANY) grid = kCUs;
+  tile_kernel<KIND, TA, TB, TA, BM, BN, WM, WN, MANY, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
   GMD_HIP(hipGetLastError());
   return GMD_OK;
 }

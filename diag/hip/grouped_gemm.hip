@@ -28,9 +28,15 @@ int launch_bf16(int op, const Args& p, hipStream_t st) {
   Args one = p;  // an expert's share of the rows is its contraction
   one.offsets = nullptr, one.k = (int)(((int64_t)p.k + p.groups - 1) / p.groups);
   const double steps = std::ceil(one.k / 64.0);
-  return TileCost::large(p.groups * tiles_of(one, 256, 256), steps) < TileCost::small(p.groups * tiles_of(one, 128, 128), steps)
-             ? launch_tile<kBf16, true, true, 256, 256, 2, 4, OUT>(p, st)
-             : launch_tile<kBf16, true, true, 128, 128, 4, 2, OUT>(p, st);
+  const double large = p.groups * tiles_of(one, 256, 256);
+  if (TileCost::large(large, steps) >= TileCost::small(p.groups * tiles_of(one, 128, 128), steps))
+    return launch_tile<kBf16, true, true, 128, 128, 4, 2, OUT>(p, st);
+  // Tiles cost what their experts have of rows.  Walked in fixed turns they save the start of a workgroup each (16 experts of 4096 x
+  // 4096, 16k rows: 447 us, 516 one by one; 32 of 2048 x 2048, 16k rows: 169 and 181), but are uneven unless an expert fills
+  // whole rounds, the rows are few, or the rounds many (16 experts of 4096 x 2048, 16k rows: 267 and 262; 8 of them, 8k rows: 140
+  // and 129; 32 of 1024 x 1024, 8k rows: 41 and 36).
+  const bool walk = large >= 256.0 * p.groups || steps <= 2 || (steps <= 8 && large >= 8 * 256);
+  return walk ? launch_tile<kBf16, true, true, 256, 256, 2, 4, OUT, true>(p, st) : launch_tile<kBf16, true, true, 256, 256, 2, 4, OUT, false>(p, st);
 }
 
 }  // namespace

@@ -436,6 +436,13 @@ def test_grouped_weight_gradient_in_large_tiles(diag, dev, rows, out, kind):
     run_grouped(diag, dev, "wgrad", "bf16", rows, 3, 1304, 2600, split(rows, 3, rows, kind), out=out)
 
 
+@pytest.mark.parametrize("kind", ["even", "random", "one", "sparse"])
+@pytest.mark.parametrize("rows,groups,n,k", [(300, 6, 2040, 2552), (600, 1, 5112, 5112)])
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_grouped_weight_gradient_walks_many_large_tiles(diag, dev, rows, groups, n, k, out, kind):
+    run_grouped(diag, dev, "wgrad", "bf16", rows, groups, n, k, split(rows, groups, 5, kind), out=out)
+
+
 @pytest.mark.parametrize("op,dtype", OPS)
 @pytest.mark.parametrize("rows,groups", [(40, 9), (600, 5), (6000, 4)])
 def test_grouped_strides_f32_results_and_rows_of_no_expert(diag, dev, op, dtype, rows, groups):
