@@ -28,8 +28,11 @@ int launch_bf16(int op, const Args& p, hipStream_t st) {
   Args one = p;  // an expert's share of the rows is its contraction
   one.offsets = nullptr, one.k = (int)(((int64_t)p.k + p.groups - 1) / p.groups);
   const double steps = std::ceil(one.k / 64.0);
-  const double large = p.groups * tiles_of(one, 256, 256);
-  if (TileCost::large(large, steps) >= TileCost::small(p.groups * tiles_of(one, 128, 128), steps))
+  // The last tile may be one of an expert with several times the average's rows (three are assumed): in one or two rounds that
+  // decides (32 experts of 976 x 496, 31k rows: small 92 us, large 114; 64 of 512 x 512, 3000 rows: 15 and 22).
+  const double large = p.groups * tiles_of(one, 256, 256), most = p.groups > 1 ? 3 * steps : steps;
+  if (std::max(TileCost::large(large, steps), TileCost::large(1, most)) >=
+      std::max(TileCost::small(p.groups * tiles_of(one, 128, 128), steps), TileCost::small(512, most)))
     return launch_tile<kBf16, true, true, 128, 128, 4, 2, OUT>(p, st);
   // Tiles cost what their experts have of rows.  Walked in fixed turns they save the start of a workgroup each (16 experts of 4096 x
   // 4096, 16k rows: 447 us, 516 one by one; 32 of 2048 x 2048, 16k rows: 169 and 181), but are uneven unless an expert fills

@@ -437,9 +437,9 @@ def test_grouped_weight_gradient_in_large_tiles(diag, dev, rows, out, kind):
 
 
 @pytest.mark.parametrize("kind", ["even", "random", "one", "sparse"])
-@pytest.mark.parametrize("rows,groups,n,k", [(300, 6, 2040, 2552), (600, 1, 5112, 5112)])
+@pytest.mark.parametrize("rows,groups,n,k", [(300, 6, 2040, 2552), (600, 1, 5112, 5112), (2000, 8, 2040, 2040)])
 @pytest.mark.parametrize("out", ["bf16", "f32"])
-def test_grouped_weight_gradient_walks_many_large_tiles(diag, dev, rows, groups, n, k, out, kind):
+def test_grouped_weight_gradient_of_many_large_tiles(diag, dev, rows, groups, n, k, out, kind):
     run_grouped(diag, dev, "wgrad", "bf16", rows, groups, n, k, split(rows, groups, 5, kind), out=out)
 
 
