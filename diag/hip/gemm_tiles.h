@@ -980,11 +980,11 @@ int launch_forward(const Args& p, hipStream_t st) {
   if constexpr (KIND == kBf16 || sizeof(OUT) == 2)
     if (large_tiles(p, KIND == kBf16 ? 64 : 128)) return launch_tile<KIND, false, false, 256, 256, 2, 4, OUT>(p, st);
   // (widening costs a wave per fragment, not per product: four waves of 64 x 64 have fewer of them per product than eight of 32 x 64,
-  // 2048 x 7168 x 8192 276 against 326 us.  With one workgroup or none on a CU four waves are too few to hide their latencies, and
+  // 2048 x 7168 x 8192 276 against 326 us.  With one workgroup or none on most CUs four waves are too few to hide their latencies, and
   // either eight are better, 3584 x 1024 x 7168 by rows 75 against 96 us, or, where it has B's scales as scalars, the few-row kernel,
-  // by tiles 65 against 89)
+  // by tiles 65 against 89; 5590 x 808 x 7248 94 and 125; 4096 x 1792 x 2048 43 and 41)
   if constexpr (KIND != kBf16 && sizeof(OUT) == 4) {
-    if (grid_of(p, 128, 128) > kCUs) return launch_tile<KIND, false, false, 128, 128, 2, 2, OUT>(p, st);
+    if (grid_of(p, 128, 128) > (KIND == kFp8Tiles ? kCUs * 3 / 2 : kCUs)) return launch_tile<KIND, false, false, 128, 128, 2, 2, OUT>(p, st);
     if constexpr (KIND == kFp8Tiles) return launch_few<KIND, false, false, 4, 4, 4, 1, OUT>(p, st);
     else return launch_tile<KIND, false, false, 128, 128, 4, 2, OUT>(p, st);
   } else {
