@@ -974,6 +974,9 @@ int launch_forward(const Args& p, hipStream_t st) {
   if (nb == 1) return launch_few<KIND, false, false, 4, 1, 6, 2, OUT>(p, st);
   if (nb == 2) return launch_few<KIND, false, false, 4, 2, 8, 1, OUT>(p, st);
   if (nb == 4) return launch_few<KIND, false, false, 4, 4, 4, 2, OUT>(p, st);
+  // (a few more than one workgroup a CU: half as large they are two on every CU, and not two on some, 203 x 4120 x 4096 12.3 against
+  // 15.0 us; with four of the half ones a CU the large ones read less, 256 x 7168 x 2048 11.9 against 14.0)
+  if (!p.offsets && grid_of(p, 64, 64) <= 2 * kCUs && grid_of(p, 32, 64) <= 2 * kCUs) return launch_few<KIND, false, false, 2, 4, 4, 1, OUT>(p, st);
   // (one slot each leaves room for two workgroups a CU)
   if (grid_of(p, 64, 64) <= 2 * kCUs) return launch_few<KIND, false, false, 4, 4, 4, 1, OUT>(p, st);
   // (f32 results of e4m3 operands are computed on widened fragments, which do not fit the large tile's registers)
