@@ -495,6 +495,22 @@ def test_grouped_offsets_up_and_down_over_many_tiles(diag, dev, op, dtype, n, k,
     assert guards_intact(raw) and bool(c.isfinite().all())
 
 
+def test_sums_over_nothing_in_large_tiles(diag, dev):
+    raw, c = guarded(5000, 5208, torch.bfloat16, dev)
+    diag.gemm_block_launch(0, 0, 0, 0, c.data_ptr(), 5000, 5208, 0, stream=_stream())
+    torch.cuda.synchronize()
+    assert guards_intact(raw) and bool((c == 0).all())
+    offsets = torch.tensor([0, 10, 10, 4000, 4900], dtype=torch.int32, device=dev)
+    raw, c = guarded(5000, 5208, torch.float32, dev)
+    diag.grouped_gemm_launch("forward", "bf16", 0, 0, c.data_ptr(), offsets.data_ptr(), 4, 5000, 5208, 0, out="f32", stream=_stream())
+    torch.cuda.synchronize()
+    assert guards_intact(raw) and bool((c[:4900] == 0).all()) and bool((c[4900:] == 7.0).all())
+    raw, c = guarded(4 * 2040, 2552, torch.float32, dev)  # experts without rows
+    diag.grouped_gemm_launch("wgrad", "bf16", 0, 0, c.data_ptr(), offsets.data_ptr(), 4, 0, 2040, 2552, out="f32", stream=_stream())
+    torch.cuda.synchronize()
+    assert guards_intact(raw) and bool((c == 0).all())
+
+
 def test_grouped_input_gradient_of_no_columns_is_zero(diag, dev):
     c = torch.full((70, 64), 7.0, dtype=torch.bfloat16, device=dev)
     offsets = torch.tensor([3, 30, 30, 66], dtype=torch.int32, device=dev)
