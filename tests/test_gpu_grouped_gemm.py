@@ -625,6 +625,45 @@ def test_chain_matches_64_bits_step_by_step(diag, dev):
     assert_product(l.dw2, *grouped_ref("wgrad", z, act, at, l.rows, l.d, l.h), l.rows)
 
 
+@pytest.mark.parametrize("rows,groups,n,k", [(37, 6, 272, 400), (900, 5, 264, 392), (6000, 3, 2064, 1104)])
+def test_training_step_of_fp8_experts(diag, dev, rows, groups, n, k):
+    """Forward, and the input gradient as a forward with the weights quantised transposed, each against 64 bits on the operands
+    it got; the weight gradient in bf16.  n and k off the block grid: what pads a quantised row is zeros."""
+    g = _gen(dev, rows)
+    at = split(rows - 5, groups, 6, "random")
+    offsets = torch.tensor(at, dtype=torch.int32, device=dev)
+    x = torch.randn(rows, k, device=dev, generator=g).bfloat16()
+    dy = torch.randn(rows, n, device=dev, generator=g).bfloat16()
+    w = torch.randn(groups, n, k, device=dev, generator=g) / math.sqrt(k)
+    e4, n16, k16 = torch.float8_e4m3fn, _up(n, 16), _up(k, 16)
+    nb, kb = _up(n, 128) // 128, _up(k, 128) // 128
+    xq, xs = torch.empty(rows, k16, dtype=e4, device=dev), torch.empty(kb, rows, device=dev)
+    dq, ds = torch.empty(rows, n16, dtype=e4, device=dev), torch.empty(nb, rows, device=dev)
+    wq, ws = torch.empty(groups, n, k16, dtype=e4, device=dev), torch.empty(groups, nb, kb, device=dev)
+    tq, ts = torch.empty(groups, k, n16, dtype=e4, device=dev), torch.empty(groups, kb, nb, device=dev)
+    st = _stream()
+    diag.block_quantize_launch(x.data_ptr(), xq.data_ptr(), xs.data_ptr(), rows, k, stream=st)
+    diag.block_quantize_launch(dy.data_ptr(), dq.data_ptr(), ds.data_ptr(), rows, n, stream=st)
+    for e in range(groups):
+        diag.block_quantize_launch(w[e].data_ptr(), wq[e].data_ptr(), ws[e].data_ptr(), n, k, dtype="f32", blocks="tiles", stream=st)
+        diag.block_quantize_launch(w[e].data_ptr(), tq[e].data_ptr(), ts[e].data_ptr(), n, k, dtype="f32", blocks="tiles", transpose=True, stream=st)
+    y, dx = torch.full((rows, n), 7.0, dtype=torch.bfloat16, device=dev), torch.full((rows, k), 7.0, device=dev)
+    dw = torch.empty(groups, n, k, device=dev)
+    diag.grouped_gemm_launch("forward", "fp8", xq.data_ptr(), wq.data_ptr(), y.data_ptr(), offsets.data_ptr(), groups, rows, n, k16,
+                             scale_a=xs.data_ptr(), scale_b=ws.data_ptr(), stream=st)
+    diag.grouped_gemm_launch("forward", "fp8", dq.data_ptr(), tq.data_ptr(), dx.data_ptr(), offsets.data_ptr(), groups, rows, k, n16, out="f32",
+                             scale_a=ds.data_ptr(), scale_b=ts.data_ptr(), stream=st)
+    diag.grouped_gemm_launch("wgrad", "bf16", dy.data_ptr(), x.data_ptr(), dw.data_ptr(), offsets.data_ptr(), groups, rows, n, k, out="f32", stream=st)
+    torch.cuda.synchronize()
+    used = at[-1]
+    for got, a, b, deep in ((y, values(xq, xs, "rows"), [values(wq[e], ws[e], "tiles") for e in range(groups)], k16),
+                            (dx, values(dq, ds, "rows"), [values(tq[e], ts[e], "tiles") for e in range(groups)], n16)):
+        ref, mag = grouped_ref("forward", a, b, at, rows, got.shape[1], deep)
+        assert_product(got[:used], ref[:used], mag[:used], deep, deep // 128 + 1)
+        assert bool((got[used:] == 7.0).all())
+    assert_product(dw, *grouped_ref("wgrad", dy.double(), x.double(), at, rows, n, k), rows)
+
+
 def test_same_results_every_time_on_any_stream_and_two_at_once(diag, dev):
     one, two = Layer(diag, dev, 900, 7, 256, 384, 2), Layer(diag, dev, 333, 20, 272, 264, 3)
     for l in (one, two):
