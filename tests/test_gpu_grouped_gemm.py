@@ -664,8 +664,9 @@ def test_training_step_of_fp8_experts(diag, dev, rows, groups, n, k):
     assert_product(dw, *grouped_ref("wgrad", dy.double(), x.double(), at, rows, n, k), rows)
 
 
-def test_same_results_every_time_on_any_stream_and_two_at_once(diag, dev):
-    one, two = Layer(diag, dev, 900, 7, 256, 384, 2), Layer(diag, dev, 333, 20, 272, 264, 3)
+@pytest.mark.parametrize("first", [(900, 7, 256, 384), (6000, 3, 4368, 2576)])
+def test_same_results_every_time_on_any_stream_and_two_at_once(diag, dev, first):
+    one, two = Layer(diag, dev, *first, 2), Layer(diag, dev, 333, 20, 272, 264, 3)
     for l in (one, two):
         l.run()
     torch.cuda.synchronize()
@@ -685,8 +686,9 @@ def test_same_results_every_time_on_any_stream_and_two_at_once(diag, dev):
             assert all(torch.equal(a, b) for a, b in zip(l.results(), w))
 
 
-def test_captured_chain_replays_on_new_inputs_and_new_offsets(diag, dev):
-    l = Layer(diag, dev, 640, 6, 256, 272, 4)
+@pytest.mark.parametrize("size", [(640, 6, 256, 272), (6000, 3, 4368, 4368)])  # (the second walks many large tiles)
+def test_captured_chain_replays_on_new_inputs_and_new_offsets(diag, dev, size):
+    l = Layer(diag, dev, *size, 4)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
