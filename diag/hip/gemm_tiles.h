@@ -134,20 +134,32 @@ struct RowTiles {
   }
 };
 
-// The weight gradient's tile with this id, and its expert's rows as the contraction.  Every XCD takes an eighth of every
-// expert's tiles, neighbours of the walk: the experts' numbers of rows differ, and with them what a tile costs (16k rows over 16
-// experts of 4096 x 2048: 305 us, with whole experts dealt to the XCDs 470).
-__device__ __forceinline__ bool wgrad_tile(const Args& p, int bm, int bn, int id, Tile* t, int64_t* k_first, int* K) {
-  const int tiles_m = (p.m + bm - 1) / bm, tiles_n = (p.n + bn - 1) / bn, eighth = (tiles_m * tiles_n + 7) / 8;
-  const int slot = id >> 3, work = (id & 7) * eighth + slot % eighth;
-  if (work >= tiles_m * tiles_n) return false;
-  int tm, tn, lo, hi;
-  tile_walk(work, tiles_m, tiles_n, &tm, &tn);
-  t->group = slot / eighth, t->m0 = tm * bm, t->m_end = p.m, t->n0 = tn * bn;
-  group_rows(p.offsets, t->group, p.k, &lo, &hi);
-  *k_first = lo, *K = hi - lo;
-  return true;
-}
+// The weight gradient's tiles, an expert's rows as the contraction of each.  Every XCD takes an eighth of every expert's tiles,
+// neighbours of the walk: the experts' numbers of rows differ, and with them what a tile costs (16k rows over 16 experts of 4096
+// x 2048: 305 us, with whole experts dealt to the XCDs 470).
+struct WgradTiles {
+  int bm, bn, tiles_m, tiles_n, eighth, ids;
+  int lo, hi;  // of expert `lane`
+
+  __device__ __forceinline__ void init(const Args& p, int bm_, int bn_) {
+    const int lane = threadIdx.x & 63;
+    bm = bm_, bn = bn_, tiles_m = (p.m + bm - 1) / bm, tiles_n = (p.n + bn - 1) / bn, eighth = (tiles_m * tiles_n + 7) / 8;
+    ids = p.groups * eighth * 8;
+    lo = hi = 0;
+    if (lane < p.groups) group_rows(p.offsets, lane, p.k, &lo, &hi);
+  }
+  __device__ __forceinline__ bool find(const Args& p, int id, Tile* t, int64_t* k_first, int* K) const {
+    const int slot = id >> 3, work = (id & 7) * eighth + slot % eighth, g = slot / eighth;
+    if (work >= tiles_m * tiles_n) return false;
+    int tm, tn, first, end;
+    tile_walk(work, tiles_m, tiles_n, &tm, &tn);
+    t->group = g, t->m0 = tm * bm, t->m_end = p.m, t->n0 = tn * bn;
+    if (g < 64) first = __builtin_amdgcn_readlane(lo, g), end = __builtin_amdgcn_readlane(hi, g);
+    else group_rows(p.offsets, g, p.k, &first, &end);
+    *k_first = first, *K = end - first;
+    return true;
+  }
+};
 
 // ------------------------------------------------------------------------------------------------------ LDS image --
 // k contiguous: 8 rows x 128 bytes per KiB, which is what one wave-wide LDS-DMA instruction of 16 bytes a lane writes,
@@ -707,12 +719,13 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
   int id = blockIdx.x;
   auto next_id = [&]() { return (id & ~(kCUs - 1)) + kCUs + ((id + 17 * 8) & (kCUs - 1)); };
   if constexpr (WGRAD) {
-    const int ids = p.groups * (((p.m + BM - 1) / BM * ((p.n + BN - 1) / BN) + 7) / 8 * 8);
+    WgradTiles tiles;
+    tiles.init(p, BM, BN);
     compute_tiles<KIND, TA, TB, WGRAD, BM, BN, WM, WN, MANY, OUT>(p, smem, [&](Tile* t, int64_t* k_first, int* K) {
       bool found = false;
-      while (!found && id < ids) {
-        found = wgrad_tile(p, BM, BN, id, t, k_first, K);
-        id = MANY ? next_id() : ids;
+      while (!found && id < tiles.ids) {
+        found = tiles.find(p, id, t, k_first, K);
+        id = MANY ? next_id() : tiles.ids;
       }
       return found;
     });
@@ -771,7 +784,9 @@ __global__ __launch_bounds__(W * 64) void few_rows_kernel(Args p) {
   int64_t k_first = 0;
   int K = p.k;
   if constexpr (kWgrad) {
-    if (!wgrad_tile(p, MB * 16, NB * 16, blockIdx.x, &t, &k_first, &K)) return;
+    WgradTiles tiles;
+    tiles.init(p, MB * 16, NB * 16);
+    if (!tiles.find(p, blockIdx.x, &t, &k_first, &K)) return;
   } else {
     RowTiles tiles;
     tiles.init(p, MB * 16, NB * 16);
@@ -894,7 +909,7 @@ inline int64_t grid_of(const Args& p, int bm, int bn) {
 inline int64_t grid_for(const Args& p, bool wgrad, int bm, int bn) {
   if (!wgrad) return grid_of(p, bm, bn);
   const int64_t tiles = (((int64_t)p.m + bm - 1) / bm) * (((int64_t)p.n + bn - 1) / bn);
-  return p.groups * ((tiles + 7) / 8 * 8);  // wgrad_tile
+  return p.groups * ((tiles + 7) / 8 * 8);  // WgradTiles
 }
 // Sizes and grids up to here: rounded up to a tile, or a round of workgroups further, they still fit 31 bits.
 constexpr int kMaxSize = 0x7fffffff - 1023;
