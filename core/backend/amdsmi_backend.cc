@@ -16,6 +16,7 @@
 #include <climits>
 #include <cstdlib>
 #include <cstring>
+#include <dirent.h>
 #include <dlfcn.h>
 #include <fcntl.h>
 #include <map>
@@ -238,6 +239,23 @@ const std::string& sysfs_root() {
 std::string sysfs_trim(const std::string& path) {
   std::string s;
   return read_file(path, &s) ? trim(s) : std::string();
+}
+
+// A microwatt file of the device's hwmon directory in W, NaN where there is none.
+double hwmon_power_w(const std::string& bdf, const char* file) {
+  const std::string dir = sysfs_root() + "/bus/pci/devices/" + bdf + "/hwmon";
+  double w = NAN;
+  if (DIR* at = opendir(dir.c_str())) {
+    while (const dirent* e = readdir(at)) {
+      if (strncmp(e->d_name, "hwmon", 5) != 0) continue;
+      const std::string v = sysfs_trim(dir + "/" + e->d_name + "/" + file);
+      char* end = nullptr;
+      const double uw = strtod(v.c_str(), &end);
+      if (end != v.c_str() && uw > 0) w = uw / 1e6;
+    }
+    closedir(at);
+  }
+  return w;
 }
 
 int pcie_gen_from_speed_dgts(uint32_t tenth_gts) {  // 0.1 GT/s units
@@ -847,16 +865,8 @@ class AmdSmiBackend : public Backend {
         if (valid(e.hip_id)) s.hip_id = (int)e.hip_id;
       }
     }
-    if (api_.amdsmi_get_power_cap_info) {
-      amdsmi_power_cap_info_t p;
-      memset(&p, 0, sizeof p);
-      if (api_.amdsmi_get_power_cap_info(d.h, 0, &p) == AMDSMI_STATUS_SUCCESS) {
-        s.power_cap_w = (double)p.power_cap / 1e6;  // µW on bare metal
-        // 0 is the library's "not reported" (seen on MI355X with ROCm 7.2), not a 0 W default.
-        if (p.default_power_cap > 0) s.power_cap_default_w = (double)p.default_power_cap / 1e6;
-        s.power_cap_max_w = (double)p.max_power_cap / 1e6;
-      }
-    }
+    PowerCap cap;
+    if (read_power_cap(d, &cap) == AMDSMI_STATUS_SUCCESS) s.power_cap_w = cap.now, s.power_cap_default_w = cap.preset, s.power_cap_max_w = cap.max;
     if (api_.amdsmi_get_gpu_memory_total) {
       uint64_t b = 0;
       if (api_.amdsmi_get_gpu_memory_total(d.h, AMDSMI_MEM_TYPE_VRAM, &b) == AMDSMI_STATUS_SUCCESS) s.vram_total_mib = (int64_t)(b >> 20);
@@ -1468,6 +1478,31 @@ class AmdSmiBackend : public Backend {
     return true;
   }
 
+  struct PowerCap { double now = NAN, preset = NAN, max = NAN; };  // W
+  // The library answers only where the driver exposes the cap with its range and default; boxes have been seen whose driver
+  // shows power1_cap alone, and that file is then read here.  Partitions of a GPU share the file: the first has the cap.
+  amdsmi_status_t read_power_cap(const Dev& d, PowerCap* cap) {
+    amdsmi_status_t rc = AMDSMI_STATUS_NOT_SUPPORTED;
+    if (api_.amdsmi_get_power_cap_info) {
+      amdsmi_power_cap_info_t p;
+      memset(&p, 0, sizeof p);
+      rc = api_.amdsmi_get_power_cap_info(d.h, 0, &p);
+      if (rc == AMDSMI_STATUS_SUCCESS) {
+        cap->now = (double)p.power_cap / 1e6;  // µW on bare metal
+        // 0 is the library's "not reported" (seen on MI355X with ROCm 7.2), not a 0 W default.
+        if (p.default_power_cap > 0) cap->preset = (double)p.default_power_cap / 1e6;
+        cap->max = (double)p.max_power_cap / 1e6;
+        return rc;
+      }
+    }
+    if (d.partition_id || d.st.pci_bdf.empty()) return rc;
+    cap->now = hwmon_power_w(d.st.pci_bdf, "power1_cap");
+    if (std::isnan(cap->now)) return rc;
+    cap->preset = hwmon_power_w(d.st.pci_bdf, "power1_cap_default");
+    cap->max = hwmon_power_w(d.st.pci_bdf, "power1_cap_max");
+    return AMDSMI_STATUS_SUCCESS;
+  }
+
   bool sample_perf(Dev& d, Sample* out) {
     bool ok = false;
     if (api_.amdsmi_get_gpu_perf_level) {
@@ -1480,16 +1515,13 @@ class AmdSmiBackend : public Backend {
         out->set_blank(GM_FI_PERF_LEVEL, blank_reason(rc == AMDSMI_STATUS_SUCCESS ? AMDSMI_STATUS_NOT_SUPPORTED : rc));
       }
     }
-    if (api_.amdsmi_get_power_cap_info) {
-      amdsmi_power_cap_info_t p;
-      memset(&p, 0, sizeof p);
-      amdsmi_status_t rc = api_.amdsmi_get_power_cap_info(d.h, 0, &p);
-      if (rc == AMDSMI_STATUS_SUCCESS) {
-        out->set_d(GM_FI_DEV_POWER_CAP, (double)p.power_cap / 1e6);
-        ok = true;
-      } else {
-        out->set_blank(GM_FI_DEV_POWER_CAP, blank_reason(rc));
-      }
+    PowerCap cap;
+    const amdsmi_status_t rc = read_power_cap(d, &cap);
+    if (rc == AMDSMI_STATUS_SUCCESS) {
+      out->set_d(GM_FI_DEV_POWER_CAP, cap.now);
+      ok = true;
+    } else if (api_.amdsmi_get_power_cap_info) {
+      out->set_blank(GM_FI_DEV_POWER_CAP, blank_reason(rc));
     }
     out->blank_untouched(SRC_PERF, GM_VS_NOT_SUPPORTED);
     return ok;

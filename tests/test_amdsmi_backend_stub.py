@@ -248,3 +248,47 @@ def test_shutdown_waits_for_the_calls_the_backend_has_inside_the_library(stub, t
     power, read_s, shutdown_s = r.stdout.split()
     assert float(power) > 0 and float(read_s) < 0.25, r.stdout    # the read did not wait for the check ...
     assert 0.05 < float(shutdown_s) < 2.0, r.stdout               # ... the shutdown did
+
+
+PROBE_POWER_CAP = r"""
+import json
+from k8s_gpu_monitor_amd import engine as E
+E.init(backend="amdsmi")
+CAP = 160  # GM_FI_DEV_POWER_CAP
+out = []
+for i in range(E.device_count()):
+    g = E.group_create(f"g{i}", [i]); fg = E.field_group_create(f"f{i}", [CAP])
+    E.watch_fields(g, fg, update_freq_us=1_000_000)
+    E.update_all_fields(True)
+    a = E.device_attributes(i)
+    nan = lambda x: None if x != x else x
+    out.append([nan(a["power_cap_w"]), nan(a["power_cap_default_w"]), E.latest_values(i, [CAP])[CAP]])
+E.shutdown()
+print(json.dumps(out))
+"""
+
+
+def test_power_cap_is_read_from_the_driver_where_the_library_gives_none(tmp_path, tables):
+    """The library wants the cap's range and default as well as the cap, and answers "not supported" on hosts whose driver shows
+    power1_cap alone (seen on MI355X): the cap is then read from the device's hwmon directory."""
+    wrapped = tmp_path / "stub.cc"
+    wrapped.write_text('#include <amd_smi/amdsmi.h>\n#define amdsmi_get_power_cap_info stub_power_cap\n'
+                       f'#include "{os.path.join(ROOT, "tests", "stubs", "amdsmi_stub.cc")}"\n#undef amdsmi_get_power_cap_info\n'
+                       'extern "C" amdsmi_status_t amdsmi_get_power_cap_info(amdsmi_processor_handle, uint32_t, amdsmi_power_cap_info_t*) '
+                       '{ return AMDSMI_STATUS_NOT_SUPPORTED; }\n')
+    lib = tmp_path / "libamd_smi_stub.so"
+    subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-I/opt/rocm/include", str(wrapped), "-o", str(lib)], check=True, timeout=120)
+    sysfs = tmp_path / "sys"
+    for i, files in enumerate(({"power1_cap": "1400000000\n"}, {"power1_cap": "1200000000", "power1_cap_default": "1400000000"}, {"power1_input": "1"},
+                               {"power1_cap": ""})):
+        dev = sysfs / "bus" / "pci" / "devices" / f"0000:{0x10 + i:02x}:00.0"
+        (dev / "hwmon" / "hwmon3").mkdir(parents=True)
+        (dev / "gpu_metrics").write_bytes(tables[0])
+        for name, text in files.items():
+            (dev / "hwmon" / "hwmon3" / name).write_text(text)
+    e = dict(os.environ, PYTHONPATH=ROOT, GPUMON_AMDSMI_LIB=str(lib), GPUMON_SYSFS_ROOT=str(sysfs), STUB_SYSFS=str(sysfs), STUB_GPUS="4",
+             GPUMON_PROC_ROOT=str(tmp_path / "noproc"))
+    e.pop("GPUMON_BACKEND", None)
+    r = subprocess.run([sys.executable, "-c", PROBE_POWER_CAP], capture_output=True, text=True, timeout=120, env=e)
+    assert r.returncode == 0, r.stderr[-800:]
+    assert json.loads(r.stdout.strip().splitlines()[-1]) == [[1400, None, 1400], [1200, 1400, 1200], [None, None, None], [None, None, None]]
