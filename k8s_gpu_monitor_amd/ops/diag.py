@@ -571,7 +571,9 @@ def block_quantize_launch(src, dst, scales, rows, cols, dtype="bf16", blocks="ro
 def gemm_block_launch(a, scale_a, b, scale_b, c, m, n, k, b_blocks="tiles", out="bf16", lda=0, ldb=0, ldc=0, ld_scale_a=0,
                       ld_scale_b=0, stream=None):
     """C[m, n] ("bf16" or "f32") = A[m, k] @ B[n, k]^T of e4m3 operands with an f32 scale per block of 128
-    (block_quantize_launch): A's blocks are rows, B's tiles or rows.  Any m, n a multiple of 8, k of 16."""
+    (block_quantize_launch): A's blocks are rows, B's tiles or rows.  Any m, n a multiple of 8, k of 16.
+    out="bf16" sums a block on the fp8 matrix instruction, which drops what lies 2^-13 below the largest product of each group of
+    eight k (at most 2^-10 of the sum of magnitudes); out="f32" keeps f32 sums, at half the rate."""
     _packed_launch("gmd_gemm_block_launch", _GEMM_BLOCK, stream, a or 0, b or 0, c or 0, scale_a or 0, scale_b or 0, lda, ldb, ldc,
                    ld_scale_a, ld_scale_b, m, n, k, BLOCKS[b_blocks], DTYPES[out], 0)
 
@@ -581,7 +583,8 @@ def grouped_gemm_launch(op, dtype, a, b, c, offsets, groups, rows, n, k, out="bf
     """One product per expert, rows sorted by expert: expert e owns rows offsets[e] .. offsets[e + 1] - 1 (int32 on the device).
     "forward": c[rows, n] = a[rows, k] w[e]^T with b = w [groups][n, k]; "dgrad": c[rows, k] = a[rows, n] w[e];
     "wgrad": c[groups][n, k] = per expert a[rows, n]^T b[rows, k].  dtype "bf16", or "fp8" (forward; e4m3 in blocks of
-    128 with scale_a per row and scale_b per tile of w).  Rows outside every expert's range are left as they were."""
+    128 with scale_a per row and scale_b per tile of w; sums as in gemm_block_launch).  Rows outside every expert's range are left as
+    they were."""
     _packed_launch("gmd_grouped_gemm_launch", _GROUPED_GEMM, stream, a or 0, b or 0, c or 0, offsets or 0, scale_a or 0, scale_b or 0,
                    lda, ldb, ldc, stride_w, ld_scale_a, ld_scale_b, stride_scale, GROUPED_OPS[op], DTYPES[dtype], DTYPES[out],
                    groups, rows, n, k, 0)

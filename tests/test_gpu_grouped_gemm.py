@@ -756,3 +756,66 @@ def test_operands_past_four_gigabytes(diag, dev):
         assert_product(dw[-1][j], DY.t()[j] @ X, DY.t()[j].abs() @ X.abs(), rows)
         assert bool((dw[:-1] == 0).all())
         del dw
+
+
+# --------------------------------------------------------------------- what the fp8 matrix instruction drops, and no more --
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("b_blocks", ["tiles", "rows"])
+@pytest.mark.parametrize("shape", [(1, 256, 4096), (20, 136, 2064), (203, 1032, 4096), (2048, 2304, 528), (5000, 5208, 272)])
+def test_gemm_block_loses_nothing_where_products_are_of_one_size(diag, dev, shape, b_blocks, out):
+    """Elements of 1 to 7.5 in magnitude: products are multiples of 2^-6 below 2^6, so none has a bit 2^-13 below the binade of
+    another; their sums over 4096 k stay under 2^18, whole numbers of 2^-6 within the 24 bits of f32; scales are powers of two, one
+    for each row.  The f32 result is the product itself, the bf16 result its nearest bf16."""
+    m, n, k = shape
+    g = _gen(dev, m + n + k)
+
+    def operand(r, blocks):
+        v = (1 + torch.randint(0, 8, (r, k), device=dev, generator=g) / 8) * torch.exp2(torch.randint(0, 3, (r, k), device=dev, generator=g).float())
+        q = (v * (2 * torch.randint(0, 2, (r, k), device=dev, generator=g) - 1)).to(torch.float8_e4m3fn)
+        kb = _up(k, 128) // 128
+        s = torch.exp2(torch.randint(-3, 4, (r if blocks == "rows" else _up(r, 128) // 128,), device=dev, generator=g).float())
+        s = (s.expand(kb, -1) if blocks == "rows" else s[:, None].expand(-1, kb)).contiguous()
+        return q, s, values(q, s, blocks)
+
+    a, sa, av = operand(m, "rows")
+    b, sb, bv = operand(n, b_blocks)
+    c = torch.full((m, n), 7.0, dtype=OUT[out], device=dev)
+    diag.gemm_block_launch(a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(), c.data_ptr(), m, n, k, b_blocks=b_blocks, out=out, stream=_stream())
+    torch.cuda.synchronize()
+    assert torch.equal(c, (av @ bv.t()).to(OUT[out]))
+
+
+@pytest.mark.parametrize("outliers", [False, True])
+@pytest.mark.parametrize("shape", [(16, 65536, 2048), (203, 4120, 2064), (1024, 1024, 2048)])
+def test_bf16_results_are_off_by_what_the_fp8_instruction_drops_on_real_data(diag, dev, shape, outliers):
+    """A bf16 result differs from the correctly rounded one by a step u with the probability |e| / u that an error e ahead of the
+    rounding carries it over a midpoint, so the mean of those differences is the mean of |e|.  It stays within what truncating every
+    product to 2^-13 of the binade of the largest of its group of eight k makes on the same data, counted out on 64 x 64 of the
+    results; a quarter is left for the sampling (some ten thousand elements that differ, and 4096 counted) and the f32 sums (1e-7)."""
+    m, n, k = shape
+    g = _gen(dev, m + k + outliers)
+
+    def quantized(x, blocks):
+        q = torch.empty(x.shape[0], k, dtype=torch.float8_e4m3fn, device=dev)
+        s = torch.empty((_up(k, 128) // 128, x.shape[0]) if blocks == "rows" else (_up(x.shape[0], 128) // 128, _up(k, 128) // 128), device=dev)
+        diag.block_quantize_launch(x.data_ptr(), q.data_ptr(), s.data_ptr(), x.shape[0], k, dtype="f32", blocks=blocks, stream=_stream())
+        return q, s, values(q, s, blocks)
+
+    x = torch.randn(m, k, device=dev, generator=g)
+    if outliers:
+        x *= torch.where(torch.rand(k, device=dev, generator=g) < 0.01, 20.0, 1.0)
+    a, sa, av = quantized(x, "rows")
+    b, sb, bv = quantized(torch.randn(n, k, device=dev, generator=g) / math.sqrt(k), "tiles")
+    c = torch.empty(m, n, dtype=torch.bfloat16, device=dev)
+    diag.gemm_block_launch(a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(), c.data_ptr(), m, n, k, stream=_stream())
+    torch.cuda.synchronize()
+    ref = av @ bv.t()
+    off = float((c.double() - ref.to(torch.bfloat16).double()).abs().mean() / ref.square().mean().sqrt())
+    i, j = torch.randint(0, m, (64,), device=dev, generator=g), torch.randint(0, n, (64,), device=dev, generator=g)
+    lost = torch.zeros(64, 64, dtype=torch.float64, device=dev)
+    for k0 in range(0, k, 128):  # (the scales of a block join its sum)
+        q = (a[i, k0:k0 + 128].double()[:, None] * b[j, k0:k0 + 128].double()[None]).unflatten(2, (-1, 8))
+        unit = torch.exp2(torch.floor(torch.log2(q.abs().amax(3, keepdim=True).clamp_min(2.0 ** -30))) - 13)
+        lost += (torch.trunc(q / unit) * unit - q).sum((2, 3)) * sa[k0 // 128, i].double()[:, None] * sb[j // 128, k0 // 128].double()[None]
+    model = float(lost.abs().mean() / ref.square().mean().sqrt())
+    assert off <= 1.25 * model + 1e-7, (off, model)
