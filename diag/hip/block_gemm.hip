@@ -47,7 +47,7 @@ int gmd_gemm_block_launch(const gmd_gemm_block_t* g, void* hip_stream) {
     if (!bad && (!p.sa || !p.sb || (((uintptr_t)p.sa | (uintptr_t)p.sb) & 3))) bad = "null or misaligned scales";
     if (!bad && (p.ld_sa < g->m || p.ld_sb > 1 << 28 || p.ld_sb < (g->b_blocks == GMD_BLOCK_TILES ? kb : g->n))) bad = "a stride of scales shorter than what it spans, or over 2^28";
   }
-  if (!bad) bad = gmd::elsewhere((hipStream_t)hip_stream, {g->a, g->b, g->c});
+  if (!bad) bad = gmd::elsewhere((hipStream_t)hip_stream, {g->a, g->b, g->c, p.sa, p.sb});
   if (bad) {
     gmd::set_error("block GEMM: %s", bad);
     return GMD_ERR_BADPARAM;

@@ -278,7 +278,7 @@ int gmd_block_quantize_launch(const gmd_block_quantize_t* q, void* hip_stream) {
   if (p.ld_src < q->cols) return refuse("a source row stride shorter than a row");
   if (p.ld_dst < c16 || p.ld_dst % 16) return refuse("a result row stride that is not a multiple of 16 or shorter than a row rounded up to 16");
   if (p.ld_scales < (q->blocks == GMD_BLOCK_ROWS ? r : kb)) return refuse("a stride of scales shorter than what it spans");
-  if (const char* bad = gmd::elsewhere((hipStream_t)hip_stream, {p.src, p.dst})) return refuse(bad);
+  if (const char* bad = gmd::elsewhere((hipStream_t)hip_stream, {p.src, p.dst, p.scales})) return refuse(bad);
   // A result that the caches would keep for the product that reads it is stored through them; a larger one is not (16384 x 7168:
   // 56.3 against 68.2 us).  32 MiB: the L2s of the eight XCDs together.
   p.stream = r * c16 > (32 << 20);

@@ -51,7 +51,7 @@ inline void span_plan(uint64_t n, uint64_t pass, unsigned max_grid, unsigned* gr
 
 // Why operands cannot be used on this stream, or null: memory of another GPU than the stream's would be read over the links
 // where peers are mapped and fault where they are not.  Host memory and what the runtime does not know are left to the caller.
-// 0.2 us for three operands, none where one device is visible.
+// Nothing is asked where one device is visible.
 inline const char* elsewhere(hipStream_t stream, std::initializer_list<const void*> operands) {
   static const bool several = [] {
     int n = 0;

@@ -93,7 +93,7 @@ int gmd_grouped_gemm_launch(const gmd_grouped_gemm_t* g, void* hip_stream) {
     if (!p.sa || !p.sb || (((uintptr_t)p.sa | (uintptr_t)p.sb) & 3)) bad = "null or misaligned scales";
     else if (p.ld_sa < g->rows || p.ld_sb > 1 << 28 || p.ld_sb < kb || p.stride_sb < (nb - 1) * p.ld_sb + kb) bad = "a stride of scales shorter than what it spans, or over 2^28";
   }
-  if (!bad) bad = gmd::elsewhere((hipStream_t)hip_stream, {g->a, g->b, g->c});
+  if (!bad) bad = gmd::elsewhere((hipStream_t)hip_stream, {g->a, g->b, g->c, g->offsets, p.sa, p.sb});
   if (bad) return refuse(bad);
   if (fp8) return launch_fp8(p, GMD_BLOCK_TILES, g->out_dtype, (hipStream_t)hip_stream);
   return g->out_dtype == GMD_DT_BF16 ? launch_bf16<__bf16>(g->op, p, (hipStream_t)hip_stream)
