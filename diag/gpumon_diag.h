@@ -198,7 +198,9 @@ GMD_API int gmd_mx_pack_scales(const void* scales_row_major, void* packed, int r
  * caller memory of the stream's device (operands on another one are refused), are asynchronous in `hip_stream`, need no
  * workspace, read nothing back to the host and can be captured into a graph.  A stride of 0 means packed; results do not
  * overlap operands.  A size of zero is no error: an empty result is left alone, a sum over nothing is zero.  Sizes up to
- * 2^31 - 1024, 2^20 experts. */
+ * 2^31 - 1024, 2^20 experts.  A product that does not fit into one launch of fewer than 2^32 threads is refused: with
+ * (rows of C + 16 experts) * (columns of C + 32) under 2^32, and for a weight gradient with experts * (128 x 128 tiles of one,
+ * rounded up to 8) under 2^23, each does. */
 typedef enum {
   GMD_BLOCK_ROWS = 0,  /* 128 consecutive elements of a row share a scale; scales[kb * ld_scales + row] */
   GMD_BLOCK_TILES = 1  /* 128 x 128 elements do;                          scales[(row / 128) * ld_scales + kb] */
@@ -230,7 +232,7 @@ GMD_API int gmd_block_quantize_launch(const gmd_block_quantize_t* q, void* hip_s
  * lies below 2^-13 of the largest of its group of eight k (at most 2^-10 of the sum of magnitudes, 1 to 3e-5 of the results' rms on
  * average); f32 results use the bf16 instruction on the widened elements, which keeps it, at half the rate.
  * Any m, n a multiple of 8, k a multiple of 16 (the last block may be partial); operands 16-byte aligned, row strides in
- * multiples of 16 bytes up to 8 MiB. */
+ * multiples of 16 bytes up to 8 MiB, ld_scale_b up to 2^28. */
 typedef struct {
   const void *a, *b;
   void* c;
@@ -255,7 +257,7 @@ GMD_API int gmd_gemm_block_launch(const gmd_gemm_block_t* g, void* hip_stream);
  * bf16: n and k in multiples of 8.  fp8 (e4m3 in blocks of 128: a's blocks are rows, w's tiles): forward only, n a multiple
  * of 8, k of 16; its input gradient is the forward with the weights quantised transposed.  Sums as in
  * gmd_gemm_block_launch (bf16 operands: f32 throughout).  Operands 16-byte
- * aligned, strides in multiples of 16 bytes, row strides up to 8 MiB. */
+ * aligned, strides in multiples of 16 bytes, row strides up to 8 MiB, ld_scale_b up to 2^28. */
 typedef enum { GMD_GROUPED_FORWARD = 0, GMD_GROUPED_DGRAD = 1, GMD_GROUPED_WGRAD = 2 } gmd_grouped_op_t;
 typedef struct {
   const void *a, *b;

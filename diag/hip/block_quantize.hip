@@ -234,20 +234,27 @@ __global__ __launch_bounds__(256) void quantize_region_kernel(QuantArgs p) {
   }
 }
 
+// In bands of src's rows where one launch would have 2^32 threads or more; a row of regions always fits (2^24 - 8 at most).
 template <typename SRC>
-int launch_quantize(const QuantArgs& p, bool tiles, bool trans, hipStream_t st) {
+int launch_quantize(QuantArgs p, bool tiles, bool trans, hipStream_t st) {
   const bool rows = !tiles && !trans;
-  const int64_t grid = rows ? (int64_t)((p.rows + (int64_t)kRowsGroup - 1) / kRowsGroup) * ((p.cols + (int64_t)kColsGroup - 1) / kColsGroup)
-                            : ((p.rows + (int64_t)127) / 128) * ((p.cols + (int64_t)127) / 128);
-  if (grid > 0x7fffffff) {
-    gmd::set_error("block quantise: too many blocks for one launch");
-    return GMD_ERR_BADPARAM;
+  const int group_r = rows ? kRowsGroup : 128, group_c = rows ? kColsGroup : 128;
+  const int64_t across = (p.cols + (int64_t)group_c - 1) / group_c, down = (p.rows + (int64_t)group_r - 1) / group_r;
+  const int64_t most = (((int64_t)1 << 32) / 256 - 1) / across;
+  for (int64_t at = 0; at < down; at += most) {
+    const int64_t n = std::min(most, down - at), first = at * group_r;
+    QuantArgs b = p;
+    b.rows = (int)std::min<int64_t>(p.rows - first, n * group_r);
+    b.src += first * p.ld_src * (int64_t)sizeof(SRC);
+    b.dst += trans ? first : first * p.ld_dst;
+    b.scales += rows ? first : trans && tiles ? first / 128 : first / 128 * p.ld_scales;
+    const unsigned grid = (unsigned)(n * across);
+    if (rows) quantize_rows_kernel<SRC><<<grid, 256, 0, st>>>(b);
+    else if (!trans) quantize_region_kernel<SRC, true, false><<<grid, 256, 0, st>>>(b);
+    else if (tiles) quantize_region_kernel<SRC, true, true><<<grid, 256, 0, st>>>(b);
+    else quantize_region_kernel<SRC, false, true><<<grid, 256, 0, st>>>(b);
+    GMD_HIP(hipGetLastError());
   }
-  if (rows) quantize_rows_kernel<SRC><<<(unsigned)grid, 256, 0, st>>>(p);
-  else if (!trans) quantize_region_kernel<SRC, true, false><<<(unsigned)grid, 256, 0, st>>>(p);
-  else if (tiles) quantize_region_kernel<SRC, true, true><<<(unsigned)grid, 256, 0, st>>>(p);
-  else quantize_region_kernel<SRC, false, true><<<(unsigned)grid, 256, 0, st>>>(p);
-  GMD_HIP(hipGetLastError());
   return GMD_OK;
 }
 

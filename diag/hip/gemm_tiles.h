@@ -915,9 +915,10 @@ inline int64_t grid_for(const Args& p, bool wgrad, int bm, int bn) {
 }
 // Sizes and grids up to here: rounded up to a tile, or a round of workgroups further, they still fit 31 bits.
 constexpr int kMaxSize = 0x7fffffff - 1023;
-inline int launched(const char* what, int64_t grid) {
-  if (grid <= 0 || grid > kMaxSize) {
-    set_error("%s: %lld workgroups do not fit into one launch", what, (long long)grid);
+// A launch holds fewer than 2^32 threads.
+inline int launched(const char* what, int64_t grid, int threads) {
+  if (grid <= 0 || grid > kMaxSize || grid * threads >= (int64_t)1 << 32) {
+    set_error("%s: %lld workgroups of %d threads do not fit into one launch", what, (long long)grid, threads);
     return GMD_ERR_BADPARAM;
   }
   return GMD_OK;
@@ -958,7 +959,7 @@ inline bool large_tiles(const Args& p, int step_k) {
 template <int KIND, bool TA, bool TB, int BM, int BN, int WM, int WN, typename OUT, bool MANY = (BM * BN >= 256 * 256)>
 int launch_tile(const Args& p, hipStream_t st) {
   int64_t grid = grid_for(p, TA, BM, BN);
-  if (int rc = launched("GEMM", grid)) return rc;
+  if (int rc = launched("GEMM", grid, MANY ? 1 : WM * WN * 64)) return rc;
   // One large tile fits a CU: that many workgroups walk the tiles (8192^3 e4m3 440 us, launched one by one 455).
   if (MANY) grid = kCUs;
   tile_kernel<KIND, TA, TB, TA, BM, BN, WM, WN, MANY, OUT><<<(unsigned)grid, WM * WN * 64, 0, st>>>(p);
@@ -968,7 +969,7 @@ int launch_tile(const Args& p, hipStream_t st) {
 template <int KIND, bool TA, bool TB, int MB, int NB, int W, int U, typename OUT>
 int launch_few(const Args& p, hipStream_t st) {
   const int64_t grid = grid_for(p, TA, MB * 16, NB * 16);
-  if (int rc = launched("GEMM", grid)) return rc;
+  if (int rc = launched("GEMM", grid, W * 64)) return rc;
   few_rows_kernel<KIND, TA, TB, MB, NB, W, U, OUT><<<(unsigned)grid, W * 64, 0, st>>>(p);
   GMD_HIP(hipGetLastError());
   return GMD_OK;

@@ -819,3 +819,19 @@ def test_bf16_results_are_off_by_what_the_fp8_instruction_drops_on_real_data(dia
         lost += (torch.trunc(q / unit) * unit - q).sum((2, 3)) * sa[k0 // 128, i].double()[:, None] * sb[j // 128, k0 // 128].double()[None]
     model = float(lost.abs().mean() / ref.square().mean().sqrt())
     assert off <= 1.25 * model + 1e-7, (off, model)
+
+
+def test_quantize_of_more_rows_than_one_launch_holds(diag, dev):
+    """2^24 workgroups of 256 threads are 2^32: such a matrix goes in bands, each with its own rows of the result and scales."""
+    rows, cols = (1 << 27) + 13, 3
+    x = torch.randn(rows, cols, device=dev, generator=_gen(dev, 31)).bfloat16()
+    q, s = torch.full((rows, 16), 0x55, dtype=torch.uint8, device=dev), torch.full((1, rows), -7.0, device=dev)
+    diag.block_quantize_launch(x.data_ptr(), q.data_ptr(), s.data_ptr(), rows, cols, stream=_stream())
+    torch.cuda.synchronize()
+    for i in range(0, rows, 1 << 24):
+        v = x[i:i + (1 << 24)].float()
+        amax = v.abs().amax(1).clamp_min(2.0 ** -96)
+        assert torch.equal(s[0, i:i + (1 << 24)], amax / torch.full_like(amax, 448.0))
+        want = (v * (torch.full_like(amax, 448.0) / amax)[:, None]).to(torch.float8_e4m3fn)
+        part = q[i:i + (1 << 24)]
+        assert torch.equal(part[:, :cols].contiguous().view(torch.float8_e4m3fn).float(), want.float()) and not bool(part[:, cols:].any())
