@@ -926,11 +926,13 @@ inline int launched(const char* what, int64_t grid, int threads) {
 
 // The K-contiguous product (forward, and every block-scaled one): which kernel.
 // `rows` is what one product has: all of them, or an expert's share on average (the host does not see the offsets).
-// * The few-row kernel gives a workgroup 16 MB x 16 NB of C with K spread over its waves.  MB covers the rows (one block of 16,
-//   two or four); NB is the smallest of 1, 2 and 4 whose grid still fits the chip at one workgroup a CU: every doubling of NB
+// * The few-row kernel gives a workgroup 16 MB x 16 NB of C with K spread over its waves.  MB is 1 up to 16 rows, 2 up to 32 and 4
+//   beyond; NB is the smallest of 1, 2 and 4 whose grid still fits the chip at one workgroup a CU: every doubling of NB
 //   halves the times A is read, but a CU without a workgroup is lost (32 x 4096 x 7168 e4m3: NB 1 9.9 us, NB 2 12.0; 32 x 7168 x
 //   2048: 8.2 and 6.0).  Past that, NB 4: up to 32 rows always, since what is read then is B, once; with more rows up to two
-//   workgroups a CU (128 x 7168 x 2048: 9.8 us, tiles 14.6; 203 x 4120 x 2064: 13.5 and 17.3; 512 x 3840 x 2048: 13.6 and 13.7).
+//   workgroups a CU (128 x 7168 x 2048: 9.8 us, tiles 14.6; 512 x 3840 x 2048: 13.6 and 13.7).  Over 32 rows two of these shapes
+//   are traded for one of 32 rows: 64 x 16 for 32 x 32, and 64 x 64 that are between one and two a CU for 32 x 64 where those are
+//   at most two a CU as well (203 x 4120 x 2064: 10.0 us, in 64 x 64 13.5, in tiles 17.3).
 // * Experts with up to 32 rows on average take it as well, in workgroups of four waves so that several fit on a CU and hide each
 //   other's start: 64 experts of 2048 x 2048 bf16 for 64 rows 43.4 us (tiles 58.5), for 2048 rows 62 (65.6).
 // * Tiles of 128 x 128 with eight waves, two workgroups a CU, or of 256 x 256, one a CU: by a model of their rounds over the
@@ -974,21 +976,25 @@ int launch_few(const Args& p, hipStream_t st) {
   GMD_HIP(hipGetLastError());
   return GMD_OK;
 }
+// Both operands by rows are one product, bf16 operands always one for each expert.
 template <int KIND, typename OUT>
 int launch_forward(const Args& p, hipStream_t st) {
+  constexpr bool kSingle = KIND != kBf16, kExperts = KIND != kFp8Rows;
   const int rows = p.offsets ? (int)(((int64_t)p.m + p.groups - 1) / p.groups) : p.m;
   const int mb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   const int nb = grid_of(p, 16 * mb, 16) <= kCUs ? 1 : grid_of(p, 16 * mb, 32) <= kCUs ? 2 : grid_of(p, 16 * mb, 64) <= kCUs ? 4 : 0;
   if (mb == 1) {
     if (nb == 1) return launch_few<KIND, false, false, 1, 1, 8, 2, OUT>(p, st);
     // (e4m3 experts: a slot less in flight leaves room for twice the workgroups, 128 experts of 2048 x 1024 for 128 rows 42 -> 34 us)
-    if (p.offsets) return KIND == kBf16 ? launch_few<KIND, false, false, 1, 2, 4, 2, OUT>(p, st) : launch_few<KIND, false, false, 1, 2, 4, 1, OUT>(p, st);
-    return nb == 2 ? launch_few<KIND, false, false, 1, 2, 4, 2, OUT>(p, st) : launch_few<KIND, false, false, 1, 4, 4, 2, OUT>(p, st);
+    if constexpr (kExperts)
+      if (!kSingle || p.offsets) return launch_few<KIND, false, false, 1, 2, 4, KIND == kBf16 ? 2 : 1, OUT>(p, st);
+    if constexpr (kSingle) return nb == 2 ? launch_few<KIND, false, false, 1, 2, 4, 2, OUT>(p, st) : launch_few<KIND, false, false, 1, 4, 4, 2, OUT>(p, st);
   }
   if (mb == 2) {
     if (nb == 1) return launch_few<KIND, false, false, 2, 1, 8, 2, OUT>(p, st);
-    if (p.offsets) return launch_few<KIND, false, false, 2, 4, 4, 1, OUT>(p, st);
-    return nb == 2 ? launch_few<KIND, false, false, 2, 2, 4, 2, OUT>(p, st) : launch_few<KIND, false, false, 2, 4, 4, 2, OUT>(p, st);
+    if constexpr (kExperts)
+      if (!kSingle || p.offsets) return launch_few<KIND, false, false, 2, 4, 4, 1, OUT>(p, st);
+    if constexpr (kSingle) return nb == 2 ? launch_few<KIND, false, false, 2, 2, 4, 2, OUT>(p, st) : launch_few<KIND, false, false, 2, 4, 4, 2, OUT>(p, st);
   }
   // (as many workgroups as 64 x 16, which reads a quarter more: 64 x 4096 x 7168 9.0 us, 10.4; 128 x 2048 x 8192 9.6 and 10.7)
   if (nb == 1) return launch_few<KIND, false, false, 2, 2, 8, 1, OUT>(p, st);
@@ -996,7 +1002,8 @@ int launch_forward(const Args& p, hipStream_t st) {
   if (nb == 4) return launch_few<KIND, false, false, 4, 4, 4, 2, OUT>(p, st);
   // (a few more than one workgroup a CU: half as large they are two on every CU, and not two on some, 203 x 4120 x 4096 12.3 against
   // 15.0 us; with four of the half ones a CU the large ones read less, 256 x 7168 x 2048 11.9 against 14.0)
-  if (!p.offsets && grid_of(p, 64, 64) <= 2 * kCUs && grid_of(p, 32, 64) <= 2 * kCUs) return launch_few<KIND, false, false, 2, 4, 4, 1, OUT>(p, st);
+  if constexpr (kSingle)
+    if (!p.offsets && grid_of(p, 32, 64) <= 2 * kCUs) return launch_few<KIND, false, false, 2, 4, 4, 1, OUT>(p, st);
   // (one slot each leaves room for two workgroups a CU)
   if (grid_of(p, 64, 64) <= 2 * kCUs) return launch_few<KIND, false, false, 4, 4, 4, 1, OUT>(p, st);
   // (f32 results of e4m3 operands are computed on widened fragments, which do not fit the large tile's registers)
