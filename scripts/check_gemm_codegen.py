@@ -72,6 +72,37 @@ def check(name, ins):
     return problems
 
 
+def _sgprs(operand):
+    m = re.match(r"s(?:(\d+)|\[(\d+):(\d+)\])$", operand)
+    return set() if not m else {int(m[1])} if m[1] else set(range(int(m[2]), int(m[3]) + 1))
+
+
+def scalar_bases_written_too_late(ins):
+    """Memory instructions whose scalar address a VALU instruction (v_readfirstlane, v_readlane, a compare) has written less than five
+    wait states before.  The compiler pads its own instructions, not those in inline asm, which the block-scaled and grouped GEMMs
+    fetch and store with."""
+    found = []
+    for i, l in enumerate(ins):
+        if not re.match(r"(global|buffer|scratch)_", l):
+            continue
+        base = set().union(*(_sgprs(o) for o in re.split(r"[,\s]+", l)[1:]))
+        states, j = 0, i - 1
+        while base and j >= 0 and states < 5:
+            op, *operands = re.split(r"[,\s]+", ins[j])
+            written = _sgprs(operands[0]) if operands else set()
+            if op.startswith("v_"):
+                if re.match(r"v_(add|addc|sub|subb|subrev|subbrev)_co_|v_mad_[iu]64|v_div_scale", op):
+                    written |= _sgprs(operands[1])  # the carry
+                if written & base:
+                    found.append((ins[j], l))
+                    break
+            elif op.startswith("s_") and not re.match(r"s_(waitcnt|cmp|bitcmp|cbranch|branch|barrier|nop|setprio|sleep)", op):
+                base -= written  # written anew by the scalar unit, which has waited for what it read
+            states += int(operands[0]) + 1 if op == "s_nop" else 1
+            j -= 1
+    return found
+
+
 def main():
     lib = sys.argv[1] if len(sys.argv) > 1 else os.path.join(ROOT, "build", "libgpumon_diag.so")
     kernels = disassemble(lib)

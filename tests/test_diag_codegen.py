@@ -38,3 +38,16 @@ def test_the_checker_sees_a_read_that_comes_too_early():
     spill = [good[0], "scratch_load_dword v1, off, off", good[0]] + good[1:]
     assert any("scratch" in p for p in cg.check("k", spill))
     assert cg.check("k", ["s_endpgm"]) == ["no MFMA found"]
+
+
+@pytest.mark.skipif(not (os.path.exists(LIB) and os.path.exists(OBJDUMP)), reason="needs the built diagnostics library and llvm-objdump")
+def test_memory_instructions_in_asm_read_scalar_addresses_that_are_there():
+    sys.path.insert(0, os.path.join(ROOT, "scripts"))
+    import check_gemm_codegen as cg
+    kernels = {k: v for k, v in cg.disassemble(LIB).items() if "tile_kernel" in k or "few_rows_kernel" in k}
+    assert len(kernels) > 80
+    assert not [(k, cg.scalar_bases_written_too_late(v)) for k, v in kernels.items() if cg.scalar_bases_written_too_late(v)]
+    late = ["v_readlane_b32 s4, v9, 3", "s_mov_b32 m0, s8", "s_nop 0", "global_load_lds_dwordx4 v1, s[4:5]"]
+    assert len(cg.scalar_bases_written_too_late(late)) == 1
+    assert not cg.scalar_bases_written_too_late(late[:1] + ["s_nop 2"] + late[1:])               # five states
+    assert not cg.scalar_bases_written_too_late(late[:1] + ["s_add_u32 s4, s0, s4"] + late[1:])  # written anew
