@@ -768,7 +768,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_kernel(Args p) {
 // are joined in LDS in the order of the waves.
 // Through LDS and not straight into registers because of the address path: it takes a quad of lanes that asks for 64
 // contiguous bytes in one cycle, but lanes of an MFMA operand are neighbours in different rows, one lane a cycle (64 rows of
-// 512 x 8192 e4m3: 21.7 us loaded directly, 9.3 this way).  64 experts of 4096 x 7168 e4m3 for 69 rows 183 us, 6.9 TB/s; one token
+// 512 x 8192 e4m3: 21.7 us loaded directly, 9.3 this way).  64 experts of 4096 x 7168 e4m3, of which 69 rows reach 38, 183 us, 6.1 TB/s; one token
 // through 4096 x 7168 5.4 us from the caches, three of which are the launch and the first step's latency.
 template <int KIND, bool TA, bool TB, int MB, int NB, int W, int U, typename OUT>
 __global__ __launch_bounds__(W * 64) void few_rows_kernel(Args p) {

@@ -34,7 +34,8 @@ DYNAMIC_LDS = [
 
 
 def demangle(names):
-    out = subprocess.run(["c++filt"], input="\n".join(names), capture_output=True, text=True, check=True).stdout
+    # c++filt does not know bf16 arguments (DF16b); written as a vendor type they print as __bf16
+    out = subprocess.run(["c++filt"], input="\n".join(names).replace("DF16b", "u6__bf16"), capture_output=True, text=True, check=True).stdout
     return out.splitlines()
 
 
