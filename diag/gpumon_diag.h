@@ -228,7 +228,8 @@ GMD_API int gmd_block_quantize_launch(const gmd_block_quantize_t* q, void* hip_s
 /* C[m, n] = sum over blocks kb of scale_a[kb][m] * scale_b(kb, n) * (sum over the block's k of A[m, k] * B[n, k])
  * A [m, k] and B [n, k] e4m3, row-major; C row-major bf16 or f32.  A's blocks are rows; B's are tiles (a weight)
  * or rows (a weight gradient: A = dy^T and B = x^T, both quantised along the tokens).
- * Sums are held in f32.  Within a block, bf16 results use the fp8 matrix instruction, which drops the part of a product that
+ * Sums are held in f32, and so is scale_a * scale_b, which is taken first: where it leaves the range of f32 the result does.
+ * Within a block, bf16 results use the fp8 matrix instruction, which drops the part of a product that
  * lies below 2^-13 of the largest of its group of eight k (at most 2^-10 of the sum of magnitudes, 1 to 3e-5 of the results' rms on
  * average); f32 results use the bf16 instruction on the widened elements, which keeps it, at half the rate.
  * Any m, n a multiple of 8, k a multiple of 16 (the last block may be partial); operands 16-byte aligned, row strides in
@@ -248,6 +249,7 @@ GMD_API int gmd_gemm_block_launch(const gmd_gemm_block_t* g, void* hip_stream);
 
 /* GEMMs grouped by expert.  Rows are sorted by expert: expert e owns rows offsets[e] .. offsets[e + 1] - 1 (int32, device
  * memory, groups + 1 of them, ascending); `rows` is the capacity, rows outside every expert's range are left as they were.
+ * Every workgroup scans the offsets, 64 experts at a time: made for hundreds of experts, and slow with tens of thousands.
  * Offsets that are out of range or descend are clamped into [0, rows] (the result is then of no use, but nothing outside the
  * operands is touched).  w is [groups][n, k].
  *   forward  c [rows, n]      = a [rows, k] times b = w:  c[t, n] = sum over k of a[t, k] * w[e][n, k]
