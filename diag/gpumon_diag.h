@@ -229,9 +229,10 @@ GMD_API int gmd_block_quantize_launch(const gmd_block_quantize_t* q, void* hip_s
  * A [m, k] and B [n, k] e4m3, row-major; C row-major bf16 or f32.  A's blocks are rows; B's are tiles (a weight)
  * or rows (a weight gradient: A = dy^T and B = x^T, both quantised along the tokens).
  * Sums are held in f32, and so is scale_a * scale_b, which is taken first: where it leaves the range of f32 the result does.
- * Within a block, bf16 results use the fp8 matrix instruction, which drops the part of a product that
- * lies below 2^-13 of the largest of its group of eight k (at most 2^-10 of the sum of magnitudes, 1 to 3e-5 of the results' rms on
- * average); f32 results use the bf16 instruction on the widened elements, which keeps it, at half the rate.
+ * Within a block, bf16 results of more than 32 rows (with experts: on average) use the fp8 matrix instruction, which drops the part
+ * of a product that lies below 2^-13 of the largest of its group of eight k (at most 2^-10 of the sum of magnitudes, 1 to 3e-5
+ * of the results' rms on average); f32 results, and bf16 ones of up to 32 rows, use the bf16 instruction on the widened elements,
+ * which keeps it, at half the rate where the matrix pipe counts.
  * Any m, n a multiple of 8, k a multiple of 16 (the last block may be partial); operands 16-byte aligned, row strides in
  * multiples of 16 bytes up to 8 MiB, ld_scale_b up to 2^28. */
 typedef struct {

@@ -572,8 +572,8 @@ def gemm_block_launch(a, scale_a, b, scale_b, c, m, n, k, b_blocks="tiles", out=
                       ld_scale_b=0, stream=None):
     """C[m, n] ("bf16" or "f32") = A[m, k] @ B[n, k]^T of e4m3 operands with an f32 scale per block of 128
     (block_quantize_launch): A's blocks are rows, B's tiles or rows.  Any m, n a multiple of 8, k of 16.
-    out="bf16" sums a block on the fp8 matrix instruction, which drops what lies 2^-13 below the largest product of each group of
-    eight k (at most 2^-10 of the sum of magnitudes); out="f32" keeps f32 sums, at half the rate."""
+    out="bf16" of more than 32 rows sums a block on the fp8 matrix instruction, which drops what lies 2^-13 below the largest product
+    of each group of eight k (at most 2^-10 of the sum of magnitudes); out="f32" keeps f32 sums, at half the rate."""
     _packed_launch("gmd_gemm_block_launch", _GEMM_BLOCK, stream, a or 0, b or 0, c or 0, scale_a or 0, scale_b or 0, lda, ldb, ldc,
                    ld_scale_a, ld_scale_b, m, n, k, BLOCKS[b_blocks], DTYPES[out], 0)
 
