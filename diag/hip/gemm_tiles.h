@@ -983,10 +983,11 @@ int launch_few(const Args& p, hipStream_t st) {
 template <int KIND, typename OUT>
 int launch_forward(const Args& p, hipStream_t st) {
   constexpr bool kSingle = KIND != kBf16, kExperts = KIND != kFp8Rows;
-  // Up to 32 rows the operands' way in is what bounds a product, and f32 sums cost nothing to 5 %: 64 experts of 4096 x 7168 for 69 rows
-  // 183.7 us (on the fp8 instruction 183.2), for 1497 rows 368 (356), 1 x 4096 x 7168 6.8 (6.6), 32 x 4096 x 7168 8.0 (7.6).  With more
-  // rows they cost 6 to 20 % of what the few-row kernel takes (128 x 7168 x 2048 9.8 and 8.9, 256 x 7168 x 2048 14.4 and 11.6)
-  // and twice the time of the tiles, so bf16 results there take the instruction.
+  // Up to 32 rows the operands' way in from memory is what bounds a product, and f32 sums cost nothing to 3 %: 64 experts of 4096 x 7168
+  // for 69 rows 183.0 us (on the fp8 instruction 182.7), for 1497 rows 349 (347), 1 x 4096 x 7168 7.44 (7.27), 32 x 4096 x 7168
+  // 9.46 (9.17); with B in the caches up to 19 % (1 x 4096 x 7168 5.4 and 4.5).  With more rows they cost 6 to 20 % of what the
+  // few-row kernel takes (128 x 7168 x 2048 9.8 and 8.9, 256 x 7168 x 2048 14.4 and 11.6) and as much again of the tiles
+  // (8192^3 986 and 437), so bf16 results there take the instruction.
   constexpr bool kWide = KIND != kBf16;
   const int rows = p.offsets ? (int)(((int64_t)p.m + p.groups - 1) / p.groups) : p.m;
   const int mb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
