@@ -866,7 +866,7 @@ class AmdSmiBackend : public Backend {
       }
     }
     PowerCap cap;
-    if (read_power_cap(d, &cap) == AMDSMI_STATUS_SUCCESS) s.power_cap_w = cap.now, s.power_cap_default_w = cap.preset, s.power_cap_max_w = cap.max;
+    if (read_power_cap(d, &cap, true) == AMDSMI_STATUS_SUCCESS) s.power_cap_w = cap.now, s.power_cap_default_w = cap.preset, s.power_cap_max_w = cap.max;
     if (api_.amdsmi_get_gpu_memory_total) {
       uint64_t b = 0;
       if (api_.amdsmi_get_gpu_memory_total(d.h, AMDSMI_MEM_TYPE_VRAM, &b) == AMDSMI_STATUS_SUCCESS) s.vram_total_mib = (int64_t)(b >> 20);
@@ -1481,7 +1481,7 @@ class AmdSmiBackend : public Backend {
   struct PowerCap { double now = NAN, preset = NAN, max = NAN; };  // W
   // The library answers only where the driver exposes the cap with its range and default; boxes have been seen whose driver
   // shows power1_cap alone, and that file is then read here.  Partitions of a GPU share the file: the first has the cap.
-  amdsmi_status_t read_power_cap(const Dev& d, PowerCap* cap) {
+  amdsmi_status_t read_power_cap(const Dev& d, PowerCap* cap, bool with_range) {
     amdsmi_status_t rc = AMDSMI_STATUS_NOT_SUPPORTED;
     if (api_.amdsmi_get_power_cap_info) {
       amdsmi_power_cap_info_t p;
@@ -1498,8 +1498,7 @@ class AmdSmiBackend : public Backend {
     if (d.partition_id || d.st.pci_bdf.empty()) return rc;
     cap->now = hwmon_power_w(d.st.pci_bdf, "power1_cap");
     if (std::isnan(cap->now)) return rc;
-    cap->preset = hwmon_power_w(d.st.pci_bdf, "power1_cap_default");
-    cap->max = hwmon_power_w(d.st.pci_bdf, "power1_cap_max");
+    if (with_range) cap->preset = hwmon_power_w(d.st.pci_bdf, "power1_cap_default"), cap->max = hwmon_power_w(d.st.pci_bdf, "power1_cap_max");
     return AMDSMI_STATUS_SUCCESS;
   }
 
@@ -1516,7 +1515,7 @@ class AmdSmiBackend : public Backend {
       }
     }
     PowerCap cap;
-    const amdsmi_status_t rc = read_power_cap(d, &cap);
+    const amdsmi_status_t rc = read_power_cap(d, &cap, false);
     if (rc == AMDSMI_STATUS_SUCCESS) {
       out->set_d(GM_FI_DEV_POWER_CAP, cap.now);
       ok = true;

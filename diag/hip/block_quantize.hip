@@ -236,7 +236,7 @@ __global__ __launch_bounds__(256) void quantize_region_kernel(QuantArgs p) {
 
 // In bands of src's rows where one launch would have 2^32 threads or more; a row of regions always fits (2^24 - 8 at most).
 template <typename SRC>
-int launch_quantize(QuantArgs p, bool tiles, bool trans, hipStream_t st) {
+int launch_quantize(const QuantArgs& p, bool tiles, bool trans, hipStream_t st) {
   const bool rows = !tiles && !trans;
   const int group_r = rows ? kRowsGroup : 128, group_c = rows ? kColsGroup : 128;
   const int64_t across = (p.cols + (int64_t)group_c - 1) / group_c, down = (p.rows + (int64_t)group_r - 1) / group_r;
