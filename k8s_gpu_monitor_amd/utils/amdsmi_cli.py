@@ -69,8 +69,7 @@ def parse(text):
     return doc
 
 
-def query(section, gpu=None, extra=(), timeout=60):
-    """Runs ``amd-smi <section> [-g gpu] --json`` and returns [{flattened fields}] per GPU."""
+def _run(section, gpu, extra, timeout):
     b = binary()
     if not b:
         raise FileNotFoundError("amd-smi not found")
@@ -79,6 +78,25 @@ def query(section, gpu=None, extra=(), timeout=60):
     if r.returncode != 0:
         raise RuntimeError(f"{' '.join(cmd)} -> {r.returncode}: {r.stderr[-400:]}")
     return [flatten(g) for g in parse(r.stdout)]
+
+
+# Where the driver hides the sensor files, ``metric`` prints N/A for what ``monitor`` still reads from the metrics table.
+_MONITOR = {"temperature.hotspot": "hotspot_temperature", "temperature.mem": "memory_temperature"}
+
+
+def query(section, gpu=None, extra=(), timeout=60):
+    """Runs ``amd-smi <section> [-g gpu] --json`` and returns [{flattened fields}] per GPU."""
+    rows = _run(section, gpu, extra, timeout)
+    if section == "metric" and any(k in r and r[k] is None for r in rows for k in _MONITOR):
+        try:
+            shown = {m.get("gpu"): m for m in reversed(_run("monitor", gpu, ["-t"], timeout))}  # (of partitions the first)
+        except (RuntimeError, ValueError, subprocess.TimeoutExpired):
+            shown = {}  # a tool without that view: what it does not say stays None
+        for r in rows:
+            for k, name in _MONITOR.items():
+                if k in r and r[k] is None:
+                    r[k] = shown.get(r.get("gpu"), {}).get(name)
+    return rows
 
 
 def device_count():

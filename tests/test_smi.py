@@ -170,3 +170,25 @@ def test_oracle_parser_on_canned_output():
     assert amdsmi_cli.parse('[{"gpu": 0, "bdf": "0000:05:00.0"}]')[0]["bdf"] == "0000:05:00.0"
     with pytest.raises(ValueError):
         amdsmi_cli.parse("no json here")
+
+
+def test_amdsmi_oracle_takes_temperatures_from_monitor_where_metric_has_none(tmp_path, monkeypatch):
+    """Hosts whose driver hides the sensor files: `amd-smi metric` prints N/A, `amd-smi monitor` the same sensors' values."""
+    tool = tmp_path / "amd-smi"
+    tool.write_text("""#!/bin/sh
+case "$1" in
+  metric) echo '{"gpu_data": [{"gpu": 0, "temperature": {"edge": "N/A", "hotspot": "N/A", "mem": {"value": 33, "unit": "C"}}},
+                              {"gpu": 1, "temperature": {"edge": "N/A", "hotspot": "N/A", "mem": "N/A"}}]}' ;;
+  monitor) if [ -e "$0.old" ]; then echo "unknown command" >&2; exit 2; fi
+           echo '[{"gpu": 0, "xcp": 0, "hotspot_temperature": {"value": 48, "unit": "C"}, "memory_temperature": {"value": 35, "unit": "C"}},
+                  {"gpu": 1, "xcp": 0, "hotspot_temperature": {"value": 51, "unit": "C"}, "memory_temperature": "N/A"}]' ;;
+esac
+""")
+    tool.chmod(0o755)
+    monkeypatch.setattr(amdsmi_cli, "binary", lambda: str(tool))
+    a, b = amdsmi_cli.query("metric")
+    assert (a["temperature.hotspot"], a["temperature.mem"], a["temperature.edge"]) == (48, 33, None)
+    assert (b["temperature.hotspot"], b["temperature.mem"]) == (51, None)
+    (tmp_path / "amd-smi.old").touch()
+    a, b = amdsmi_cli.query("metric")
+    assert a["temperature.hotspot"] is None and b["temperature.hotspot"] is None
